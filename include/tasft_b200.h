@@ -141,6 +141,72 @@ typedef struct {
 } tasft_qkv_args;
 TASFT_API int tasft_qkv_rope_pool(const tasft_qkv_args* args, tasft_stream_t stream);
 
+/* Rotary embedding of new tokens on their way into a paged KV cache: the packed rows of a
+ * serving step (cu_seqlens, as in tasft_bsa_chunk_paged_fwd) are rotated at their positions
+ * kv_len[b] - new + i, q to q_out, k and v into the pages, and the fp32 block means that
+ * AttnGate pools are kept: pooled_q of the new queries (row i: the i-th 64-token block that the
+ * sequence's new tokens touch, zero where there is none) and pooled_k of every key block that
+ * got new tokens (over all its rows in the cache; other rows of pooled_k are left alone). A
+ * pair (x, y) turns by position * inv_freq[i] (fp64): (x cos - y sin, y cos + x sin) * factor;
+ * pairs are (i, i + rot/2) or, interleaved, (2i, 2i + 1) of the first rot columns; fp32
+ * arithmetic, rounded once. The paged, packed counterpart of tasft_qkv_rope_pool, with other
+ * layouts and scaled frequencies; the reference has neither a paged cache nor these
+ * (tasft/modules/tasft_attention.py:872-908 takes cos and sin as given).
+ * q_out may be q. f32 / bf16 / f16; D and rot multiples of two 16-byte vectors (16 columns, 8 in
+ * f32), D <= 256; rows on 16-byte boundaries. TASFT_DEVERR_INDEX: a page out of range (its
+ * rows are not written) or a sequence whose lengths do not fit T, max_q, each other or the
+ * table (left out). A page must not be written through two sequences in one call. */
+typedef struct {
+  const void* q;            /* [T, Hq, D] */
+  const void* k;            /* [T, Hk, D] */
+  const void* v;            /* [T, Hk, D] */
+  void* q_out;              /* [T, Hq, D] */
+  void* k_pages;            /* [num_pages, page_size, Hk, D] */
+  void* v_pages;
+  int64_t q_stride[2], k_in_stride[2], v_in_stride[2], o_stride[2];  /* token, head (elements) */
+  int64_t k_stride[4], v_stride[4];                                   /* of the pages */
+  const void* inv_freq;     /* [rot / 2] radians per position, fp64 (freq_f64) or fp32 */
+  const int32_t* block_table; /* [B, max_pages] */
+  const int32_t* cu_seqlens;  /* [B + 1] ascending */
+  const int32_t* kv_len;      /* [B] tokens of each sequence, the new ones included */
+  float* pooled_q;          /* out [B, Hq, NBq, D] or NULL */
+  float* pooled_k;          /* in/out [B, Hk, NBk, D] or NULL */
+  double factor;            /* on cos and sin (attention scaling of long-context variants) */
+  int32_t B, T, Hq, Hk, D, rot, block, dtype;
+  int32_t max_q;            /* most new tokens of a sequence */
+  int32_t max_pages, page_size, num_pages;
+  int32_t NBq, NBk;         /* NBq at least (max_q + 126) / 64 */
+  int32_t interleaved, freq_f64;
+  int32_t* err;
+} tasft_rope_append_args;
+TASFT_API int tasft_rope_append_paged(const tasft_rope_append_args* args, tasft_stream_t stream);
+
+/* Kept blocks by score, for the new tokens of a packed batch: row i of sequence b stands for
+ * block mine = (kv_len[b] - new) / block + i and keeps blocks [0, first), (mine - local, mine]
+ * and the best-scored of the others below, top_k in all (the first and last ones stay even
+ * where they are more). A block's score is the highest of its group's query heads; ties go to the
+ * lowest index; NaN counts as -inf, which is never chosen; with use_tau only scores >= tau
+ * are. Ascending lists, -1 padded, for tasft_bsa_chunk_paged_fwd (or, one row per sequence,
+ * the decode calls); a row that no new token falls in keeps nothing. Beside
+ * tasft_mask_from_scores: a count instead of a threshold. The reference has no top-k
+ * (tasft/modules/attn_gate.py:475). TASFT_DEVERR_INDEX: lengths that do not fit NBq, NBk
+ * or each other (the sequence keeps nothing). NBk <= 16384. */
+typedef struct {
+  const float* scores;      /* [B, Hq, NBq, NBk] */
+  int64_t stride[3];        /* batch, head, row (elements); columns contiguous */
+  const int32_t* cu_seqlens;  /* [B + 1] */
+  const int32_t* kv_len;      /* [B] */
+  int32_t B, Hq, Hk, NBq, NBk, block;
+  int32_t top_k, first, local;
+  int32_t use_tau;
+  float tau;
+  int32_t width;            /* entries per list, at least min(NBk, max(top_k, first + local)) */
+  int32_t* kept_idx;        /* out [B, Hk, NBq, width] */
+  int32_t* kept_cnt;        /* out [B, Hk, NBq] */
+  int32_t* err;
+} tasft_select_args;
+TASFT_API int tasft_select_blocks(const tasft_select_args* args, tasft_stream_t stream);
+
 /* Threshold given fp32 scores: hard = (soft >= tau) (& block tril when causal),
  * ascending kept lists, counts and the total. Bit-exact with the reference's
  * `soft >= tau` on the same scores. */
@@ -287,6 +353,50 @@ typedef struct {
   int32_t num_pages;
 } tasft_paged_decode_args;
 TASFT_API int tasft_bsa_decode_paged_fwd(const tasft_paged_decode_args* args, tasft_stream_t stream);
+
+/* Attention of a chunk of new tokens over a paged KV cache: the new tokens of B sequences,
+ * packed along the token axis, attend causally over everything their sequence has in the
+ * cache, themselves included (their K and V are in the pages already, see
+ * tasft_rope_append_paged). Chunks of prompts and single tokens may stand in one batch. No
+ * counterpart in the reference: its vLLM backend flattens prefill tokens into one sequence
+ * without a cache (tasft/inference/vllm_patch.py:172-196).
+ * Sequence b: rows [cu_seqlens[b], cu_seqlens[b+1]) of q and out, the last of its kv_len[b]
+ * tokens. Logical token t lives in page block_table[b, t / page_size] at row t % page_size.
+ * Kept lists: row i of sequence b is the i-th 64-token block that its new tokens touch
+ * (block (kv_len[b] - new) / 64 + i), ascending block indices; entries past the row's own
+ * block keep nothing. kept_idx == NULL: every block. A token with nothing kept gets 0.
+ * Rows of out outside all sequences are left as they are.
+ * bf16 / f16, D 64 or 128, block 64, page_size 16, 32, 64 or 128, Hq / Hk <= 64; pointers and
+ * strides of whole 16 bytes. Reported in *err without a fault: TASFT_DEVERR_INDEX (a page or
+ * kept block out of range: skipped; a sequence whose lengths do not fit T, max_q, each other
+ * or the table: its rows are left out), TASFT_DEVERR_ORDER (a list that does not ascend: the
+ * entry is skipped). Cache rows from kv_len on are never used, whatever they hold. */
+typedef struct {
+  const void* q;            /* [T, Hq, D] */
+  const void* k_pages;      /* [num_pages, page_size, Hk, D] */
+  const void* v_pages;
+  void* out;                /* [T, Hq, D] */
+  int64_t q_stride[2];      /* token, head (elements) */
+  int64_t o_stride[2];
+  int64_t k_stride[4], v_stride[4];
+  const int32_t* block_table; /* [B, max_pages] */
+  const int32_t* cu_seqlens;  /* [B + 1] ascending */
+  const int32_t* kv_len;      /* [B] tokens of each sequence, the new ones included */
+  const int32_t* kept_idx;    /* [B, Hm, nb_q, nb_w] or NULL */
+  const int32_t* kept_cnt;    /* [B, Hm, nb_q] */
+  int32_t B, T, Hq, Hk, D, block, dtype;
+  int32_t max_q;            /* most new tokens of a sequence */
+  int32_t max_pages, page_size, num_pages;
+  int32_t Hm;               /* heads of the lists: Hk (one list per group) or Hq */
+  int32_t nb_q, nb_w;       /* rows per head, at least (max_q + 126) / 64; entries per row */
+  float scale;              /* softmax scale, > 0 */
+  void* workspace;          /* tasft_chunk_workspace_size() bytes */
+  int64_t workspace_bytes;
+  int32_t* err;
+} tasft_chunk_args;
+TASFT_API int64_t tasft_chunk_workspace_size(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q,
+                                             int32_t Hm);  /* Hm 0: no lists */
+TASFT_API int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* args, tasft_stream_t stream);
 
 /* Merge G partial results (normalised o, m, l) into the final output. */
 typedef struct {

@@ -21,6 +21,7 @@ from tasft_b200.block_sparse_fa import (
     detect_kernels,
     mask_to_kept,
 )
+from tasft_b200.chunk import bsa_chunk_paged, chunk_rows, rope_append_paged, rope_inv_freq, select_blocks
 from tasft_b200.decode import DecodeWorkspace, bsa_decode, bsa_decode_paged, decode_combine
 from tasft_b200.exceptions import KernelError, NaNDetectedError, TASFTError, ValidationError
 from tasft_b200.patch import patch, unpatch
@@ -51,9 +52,11 @@ __all__ = [
     "TASFTError",
     "TASFTObjective",
     "ValidationError",
+    "bsa_chunk_paged",
     "bsa_decode",
     "calibrate_tau",
     "bsa_decode_paged",
+    "chunk_rows",
     "decode_combine",
     "detect_kernels",
     "gate_losses",
@@ -64,6 +67,9 @@ __all__ = [
     "measured_sparsity_profile",
     "patch",
     "qkv_rope_pool",
+    "rope_append_paged",
+    "rope_inv_freq",
+    "select_blocks",
     "shards",
     "threshold_scores",
     "training_attention",

@@ -5,6 +5,7 @@ fallback: if the shared object is missing or fails to load, every op raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from pathlib import Path
@@ -113,6 +114,44 @@ class PagedDecodeArgs(C.Structure):
     ]
 
 
+I64x2 = C.c_int64 * 2
+
+
+class RopeAppendArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("q_out", vp), ("k_pages", vp), ("v_pages", vp),
+        ("q_stride", I64x2), ("k_in_stride", I64x2), ("v_in_stride", I64x2), ("o_stride", I64x2),
+        ("k_stride", I64x4), ("v_stride", I64x4), ("inv_freq", vp), ("block_table", vp), ("cu_seqlens", vp),
+        ("kv_len", vp), ("pooled_q", vp), ("pooled_k", vp), ("factor", C.c_double),
+        ("B", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32), ("rot", C.c_int32),
+        ("block", C.c_int32), ("dtype", C.c_int32), ("max_q", C.c_int32), ("max_pages", C.c_int32),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32), ("NBq", C.c_int32), ("NBk", C.c_int32),
+        ("interleaved", C.c_int32), ("freq_f64", C.c_int32), ("err", vp),
+    ]
+
+
+class SelectArgs(C.Structure):
+    _fields_ = [
+        ("scores", vp), ("stride", I64x3), ("cu_seqlens", vp), ("kv_len", vp),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("NBq", C.c_int32), ("NBk", C.c_int32),
+        ("block", C.c_int32), ("top_k", C.c_int32), ("first", C.c_int32), ("local", C.c_int32),
+        ("use_tau", C.c_int32), ("tau", C.c_float), ("width", C.c_int32), ("kept_idx", vp), ("kept_cnt", vp),
+        ("err", vp),
+    ]
+
+
+class ChunkArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k_pages", vp), ("v_pages", vp), ("out", vp), ("q_stride", I64x2), ("o_stride", I64x2),
+        ("k_stride", I64x4), ("v_stride", I64x4), ("block_table", vp), ("cu_seqlens", vp), ("kv_len", vp),
+        ("kept_idx", vp), ("kept_cnt", vp),
+        ("B", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32),
+        ("block", C.c_int32), ("dtype", C.c_int32), ("max_q", C.c_int32), ("max_pages", C.c_int32),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32), ("Hm", C.c_int32), ("nb_q", C.c_int32),
+        ("nb_w", C.c_int32), ("scale", C.c_float), ("workspace", vp), ("workspace_bytes", C.c_int64), ("err", vp),
+    ]
+
+
 class CombineArgs(C.Structure):
     _fields_ = [
         ("part_o", vp), ("part_ml", vp), ("G", C.c_int32), ("rows", C.c_int64), ("D", C.c_int32),
@@ -176,6 +215,10 @@ SIGNATURES = {
     "tasft_gate_mask_build": ([C.POINTER(GateArgs), vp], C.c_int),
     "tasft_mask_from_scores": ([C.POINTER(ThresholdArgs), vp], C.c_int),
     "tasft_qkv_rope_pool": ([C.POINTER(QkvArgs), vp], C.c_int),
+    "tasft_rope_append_paged": ([C.POINTER(RopeAppendArgs), vp], C.c_int),
+    "tasft_select_blocks": ([C.POINTER(SelectArgs), vp], C.c_int),
+    "tasft_chunk_workspace_size": ([C.c_int32] * 7, C.c_int64),
+    "tasft_bsa_chunk_paged_fwd": ([C.POINTER(ChunkArgs), vp], C.c_int),
     "tasft_mask_to_kept": ([C.POINTER(MaskArgs), vp], C.c_int),
     "tasft_calibrate_tau": ([C.POINTER(CalibArgs), vp], C.c_int),
     "tasft_bsa_prefill_fwd": ([C.POINTER(PrefillArgs), vp], C.c_int),
@@ -260,6 +303,13 @@ def strides3(t: torch.Tensor):
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(t: torch.Tensor):
+    """Context in which t's device is the current one (launches go to the current device)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def require_cuda(*ts: torch.Tensor) -> None:

@@ -1,0 +1,997 @@
+// Attention of a chunk of new tokens over a paged KV cache on the 5th-generation tensor cores.
+//
+// For token t at position p of its sequence and query head h of kv-head g,
+//   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q.k_j,  m = max_j s_j,
+// over the kept keys j <= p: one pass over the keys with the running (m, sum, o) of the
+// online softmax in fp32. P is rounded to the value dtype for P.V, as the prefill does.
+//
+// Tile = 128 rows that share one kv-head, filled by mode:
+//   0  every block kept: all query heads of a group times as many tokens as fit
+//      (row = token * heads + head), so a single token of a group of 4 is 4 rows
+//   1  lists per kv-head: the same, with a power of two of tokens that divides 64 and starts
+//      at its multiples, so a tile has one list
+//   2  lists per query head: two 64-token slots, two heads of a group at one 64-token block
+//      (one head at two blocks where a group has one head); the tile walks the union of the
+//      two lists and each entry says which slots keep it
+// A work item is a tile, or where few tiles face many blocks a slice of a tile's blocks; the
+// slices' (m, l, O) meet in chunk_merge_kernel. Every CTA computes the same cut from cu_seqlens
+// and kv_len, so the host needs neither.
+//
+// Persistent CTAs (2 per SM, 256 threads) take items in a static, snaking stride. Warps:
+//   0     producer: Q of the tile, then K and V of every entry through separate 2-stage rings
+//         (TMA from the pages, 128B swizzle)
+//   1     MMA issuer: S = Q K^T (SS, M128 N64) into a double-buffered TMEM tile, O += P V (TS:
+//         P read from TMEM where it overwrote S)
+//   2     lists: the next segment (at most kSeg entries) of block indices with their pages,
+//         double-buffered, ahead of the producer
+//   3     idle: warps 0-3 hand registers to the second warpgroup (128 -> 96 and 160 a thread)
+//   4-7   softmax, one thread per row; epilogue
+// Rows of V that no key stands for (past kv_len, or of a page that is not there) are zeroed in
+// shared memory before P.V, so what the cache holds there never meets a 0 of P.
+// Every mbarrier phase is indexed by a global counter and every wait is arranged so the waiter
+// is at most one phase behind; every wait is bounded (TASFT_DEVERR_TIMEOUT).
+#include "chunk.cuh"
+#include "tc.cuh"
+
+namespace tasft {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSeg = 128;                  // entries of a list segment
+constexpr uint32_t kTmemCols = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+
+// entry of a list segment: block index, which of its (up to four) pages are there, slots
+constexpr int kKbBits = 20;
+constexpr int kKbMask = (1 << kKbBits) - 1;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+  return ((uint64_t)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+}
+__device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_f(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// One list segment and the tile it belongs to.
+struct Work {
+  int n;            // entries; -1: no more work
+  int first, last;  // of the item's segments
+  int len;          // tokens of the sequence
+  int part;         // slot of the item's partials, or -1: the item is the whole tile
+  int hk;
+  // rows, by slot (modes 0 and 1 use slot 0 alone)
+  int valid[2];     // mode 0/1: tokens of the tile in [0]; mode 2: whether the slot is used
+  int head[2];      // first query head
+  int pos[2];       // position of row 0 of the slot
+  int row[2];       // its row in q and out (mode 2: of position pos, maybe before the sequence)
+  int ctx;
+};
+
+template <int D>
+struct Smem {
+  static constexpr int kChunks = D / 64;                  // 64-element (128 B) swizzle atoms along D
+  static constexpr int kQBytes = kChunks * 128 * 128;
+  static constexpr int kKVTileBytes = kChunks * 64 * 128;
+  static constexpr int kKOff = 0;
+  static constexpr int kVOff = 2 * kKVTileBytes;
+  static constexpr int kQOff = 0;
+  static constexpr int kStageOff = kQOff + kQBytes;
+  static constexpr int kListOff = kStageOff + 4 * kKVTileBytes;  // [2][kSeg] entries
+  static constexpr int kPageOff = kListOff + 2 * kSeg * 4;       // [2][kSeg][4] pages
+  static constexpr int kItemOff = kPageOff + 2 * kSeg * 16;      // [kChunkBuckets + 1] first item
+  static constexpr int kSlotOff = kItemOff + (kChunkBuckets + 1) * 4;  // the same, first split slot
+  static constexpr int kBitmapOff = kSlotOff + (kChunkBuckets + 1) * 4;  // [2][kSeg / 32]
+  static constexpr int kWorkOff = (kBitmapOff + 2 * (kSeg / 32) * 4 + 7) / 8 * 8;
+  static constexpr int kBarOff = (kWorkOff + 2 * (int)sizeof(Work) + 7) / 8 * 8;
+  static constexpr int kNumBars = 22;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kBytes = kMiscOff + 16;
+  static constexpr int kAlloc = kBytes + 1024;  // slack for 1024-byte alignment
+};
+
+struct PagedGeo {
+  int nsub;       // pages of a block (page_size < 64)
+  int sub_rows;   // rows of a page's share of a block
+};
+
+template <int D, bool kF16>
+__global__ void __launch_bounds__(kThreads, 2)
+    bsa_chunk_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                        const __grid_constant__ CUtensorMap tmv, const tasft_chunk_args a, const ChunkShape sh,
+                        const ChunkWs ws) {
+  using L = Smem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sQ = smem + L::kQOff;
+  int32_t* lists = reinterpret_cast<int32_t*>(smem + L::kListOff);
+  int4* pages = reinterpret_cast<int4*>(smem + L::kPageOff);
+  Work* works = reinterpret_cast<Work*>(smem + L::kWorkOff);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* q_full = bars + 0;       // per tile: Q landed
+  uint64_t* q_empty = bars + 1;      // per tile: every S of the tile has run (Q reusable)
+  uint64_t* k_full = bars + 2;       // [2] per block
+  uint64_t* k_empty = bars + 4;      // [2] per block: S(g) has run
+  uint64_t* s_full = bars + 6;       // [2] per block
+  uint64_t* p_ready = bars + 8;      // [2] per block (128 arrivals)
+  uint64_t* pv_done = bars + 10;     // [2] per block: P.V(g) has run
+  uint64_t* o_final = bars + 12;     // per tile: O complete
+  uint64_t* o_free = bars + 13;      // per tile: epilogue has read O (128 arrivals)
+  uint64_t* list_full = bars + 14;   // [2] per segment
+  uint64_t* list_empty = bars + 16;  // [2] per segment (128 arrivals)
+  uint64_t* v_full = bars + 18;      // [2] per block
+  uint64_t* v_empty = bars + 20;     // [2] per block: P.V(g) has run
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grp = a.Hq / a.Hk;
+
+  if (warp == 0 && lane == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 128);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&list_full[i], 1);
+      mbar_init(&list_empty[i], 128);
+    }
+    mbar_init(o_final, 1);
+    mbar_init(o_free, 128);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&misc[0], kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  // the merge kernel behind this one waits for this grid before it reads anything
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = misc[0];
+  const uint32_t tS0 = tmem;       // S buffers: columns [0,64) and [64,128)
+  const uint32_t tO = tmem + 128;  // O: columns [128, 128 + D)
+
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+
+  if (warp == 2) {
+    // ================= lists =================
+    int32_t* item0 = reinterpret_cast<int32_t*>(smem + L::kItemOff);
+    int32_t* slot0 = reinterpret_cast<int32_t*>(smem + L::kSlotOff);
+    uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + L::kBitmapOff);
+    // ---- cut the batch into items: pieces of about the mean load of a CTA ----
+    float load = 0.f;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + lane;
+      if (b < a.B) {
+        const ChunkSeq s = chunk_seq(a, sh, b);
+        load += (float)s.tiles * (float)s.cost;
+        if (s.bad && blockIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
+      }
+    }
+    load = warp_sum(load) * (float)sh.units;
+    const int target = max(kChunkMinPiece, (int)ceilf(load / (float)gridDim.x));
+    int items = 0, slots = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + lane;
+      int it = 0, sl = 0, ns = 1;
+      if (b < a.B) {
+        const ChunkSeq s = chunk_seq(a, sh, b);
+        ns = chunk_splits(s, target);
+        it = s.tiles * sh.units;
+        sl = ns > 1 ? it * ns : 0;
+      }
+      // slots count what every sequence asks for; from the first that finds no room in the
+      // workspace on, sequences stay whole
+      const int fs = warp_scan_int(sl, lane);
+      if (slots + fs > sh.slots) ns = 1;
+      const int fi = warp_scan_int(it * ns, lane);
+      if (b < a.B) {
+        if (b % sh.stride == 0) {
+          item0[b / sh.stride] = items + fi - it * ns;
+          slot0[b / sh.stride] = slots + fs - sl;
+        }
+        if (blockIdx.x == 0) ws.plan[b] = make_int2(ns, slots + fs - sl);
+      }
+      items += __shfl_sync(0xffffffffu, fi, 31);
+      slots += __shfl_sync(0xffffffffu, fs, 31);
+    }
+    __syncwarp();
+    const int buckets = (a.B + sh.stride - 1) / sh.stride;
+    const PagedGeo geo = {max(1, kChunkBlk / a.page_size), min(kChunkBlk, a.page_size)};
+
+    int u = 0;  // segment counter
+    bool ok = true;
+    for (int v = 0; ok; ++v) {
+      // the CTA order snakes (0..G-1, then G-1..0, ...), heavy tiles of a sequence first
+      const int item = v * gridDim.x + ((v & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+      Work w;
+      int lo = 0, hi = 0;                 // range of the item: list positions, or blocks
+      const int32_t* idx[2] = {nullptr, nullptr};
+      int cnt[2] = {0, 0}, qb[2] = {0, 0};
+      int b = 0;
+      const bool done = item >= items;
+      if (!done) {
+        int bl = 0, bh = buckets - 1;
+        while (bl < bh) {  // last bucket that starts at or before the item
+          const int mid = (bl + bh + 1) >> 1;
+          if (item0[mid] <= item) bl = mid;
+          else bh = mid - 1;
+        }
+        b = bl * sh.stride;
+        int first_item = item0[bl], first_slot = slot0[bl];
+        ChunkSeq s;
+        int ns;
+        while (true) {
+          s = chunk_seq(a, sh, b);
+          ns = chunk_splits(s, target);
+          const int it = s.tiles * sh.units, ask = ns > 1 ? it * ns : 0;
+          if (first_slot + ask > sh.slots) ns = 1;
+          if (item < first_item + it * ns || b + 1 >= a.B) break;
+          first_item += it * ns;
+          first_slot += ask;
+          ++b;
+        }
+        int rest = item - first_item;
+        const int unit = rest % sh.units;
+        rest /= sh.units;
+        const int split = rest % ns;
+        const int tile = s.tiles - 1 - rest / ns;
+        w.len = s.len;
+        w.ctx = s.ctx;
+        w.part = ns > 1 ? first_slot + (tile * sh.units + unit) * ns + split : -1;
+        int diag;  // last block the tile may visit
+        if (sh.mode == 2) {
+          const int base = (s.ctx / sh.tpt + tile) * sh.tpt;
+          if (grp >= 2) {
+            const int pairs = (grp + 1) / 2, p = unit % pairs;
+            w.hk = unit / pairs;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              w.head[x] = w.hk * grp + 2 * p + x;
+              w.valid[x] = 2 * p + x < grp;
+              w.pos[x] = base;
+            }
+          } else {
+            w.hk = unit;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              w.head[x] = unit;
+              w.pos[x] = base + x * kChunkBlk;
+              w.valid[x] = w.pos[x] < s.len && w.pos[x] + kChunkBlk > s.ctx;
+            }
+          }
+          diag = 0;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            w.row[x] = s.start + w.pos[x] - s.ctx;
+            qb[x] = w.pos[x] / kChunkBlk;
+            if (!w.valid[x]) continue;
+            diag = max(diag, qb[x]);
+            const int64_t lrow =
+                ((int64_t)b * a.Hm + w.head[x] / (a.Hq / a.Hm)) * a.nb_q + (qb[x] - s.ctx / kChunkBlk);
+            cnt[x] = min(max(a.kept_cnt[lrow], 0), a.nb_w);
+            idx[x] = a.kept_idx + lrow * a.nb_w;
+          }
+          // slices by block index
+          lo = (int)((int64_t)split * (diag + 1) / ns);
+          hi = (int)((int64_t)(split + 1) * (diag + 1) / ns);
+        } else {
+          w.hk = unit;
+          w.head[0] = w.head[1] = unit * grp;
+          int p0, p1;
+          if (sh.mode == 0) {
+            p0 = s.ctx + tile * sh.tpt;
+            p1 = min(p0 + sh.tpt, s.len);
+          } else {
+            p0 = (s.ctx / sh.tpt + tile) * sh.tpt;
+            p1 = min(p0 + sh.tpt, s.len);
+            p0 = max(p0, s.ctx);
+          }
+          w.valid[0] = p1 - p0;
+          w.valid[1] = 0;
+          w.pos[0] = w.pos[1] = p0;
+          w.row[0] = w.row[1] = s.start + p0 - s.ctx;
+          diag = (p1 - 1) / kChunkBlk;
+          qb[0] = diag;
+          cnt[0] = diag + 1;
+          if (sh.mode == 1) {
+            const int64_t lrow = ((int64_t)b * a.Hm + unit) * a.nb_q + (diag - s.ctx / kChunkBlk);
+            cnt[0] = min(max(a.kept_cnt[lrow], 0), a.nb_w);
+            idx[0] = a.kept_idx + lrow * a.nb_w;
+          }
+          lo = (int)((int64_t)split * cnt[0] / ns);
+          hi = (int)((int64_t)(split + 1) * cnt[0] / ns);
+        }
+      }
+      // ---- the item's segments ----
+      int at = lo;                       // next list position or block
+      int pt[2] = {0, 0};                // mode 2: next position of each list
+      int prev[2] = {-1, -1};            // last accepted block of each list
+      if (!done && sh.mode == 1 && lo > 0) prev[0] = idx[0][lo - 1];
+      bool first = true;
+      while (ok) {
+        const int lb = u & 1;
+        if (u >= 2 && !warp_wait(&list_empty[lb], ((u >> 1) - 1) & 1)) {
+          set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 9));
+          ok = false;
+          break;
+        }
+        int32_t* list = lists + lb * kSeg;
+        int4* pgs = pages + lb * kSeg;
+        if (done) {
+          if (lane == 0) {
+            works[lb].n = -1;
+            mbar_arrive(&list_full[lb]);
+          }
+          break;
+        }
+        int n = 0;
+        // ---- block indices (with slots in mode 2) ----
+        if (sh.mode == 2) {
+          const int wend = min(at + kSeg, hi);
+          if (lane < 2 * (kSeg / 32)) bitmap[lane] = 0;
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            while (pt[x] < cnt[x]) {
+              const int i = pt[x] + lane;
+              const int kb = i < cnt[x] ? idx[x][i] : INT32_MAX;
+              int before = __shfl_up_sync(0xffffffffu, kb, 1);
+              if (lane == 0) before = prev[x];
+              const bool mine = kb < wend;  // this window's (a list ascends, so a prefix)
+              const unsigned out = __ballot_sync(0xffffffffu, !mine);
+              const int take = out ? __ffs(out) - 1 : 32;
+              if (lane < take) {
+                if (kb < 0) set_err(a.err, TASFT_DEVERR_INDEX);
+                else if (kb <= before) set_err(a.err, TASFT_DEVERR_ORDER);
+                else if (kb >= at && kb <= qb[x])
+                  atomicOr(&bitmap[x * (kSeg / 32) + ((kb - at) >> 5)], 1u << ((kb - at) & 31));
+              }
+              if (take > 0) prev[x] = __shfl_sync(0xffffffffu, kb, take - 1);
+              pt[x] += take;
+              if (take < 32) break;
+            }
+          }
+          __syncwarp();
+          for (int wd = 0; wd < kSeg / 32; ++wd) {
+            const uint32_t m0 = bitmap[wd], m1 = bitmap[kSeg / 32 + wd], bit = 1u << lane;
+            const bool any = ((m0 | m1) & bit) != 0;
+            const unsigned bal = __ballot_sync(0xffffffffu, any);
+            if (any)
+              list[n + __popc(bal & (bit - 1u))] =
+                  (at + wd * 32 + lane) | (((m0 & bit) ? 1 : 0) << (kKbBits + 4)) | (((m1 & bit) ? 1 : 0) << (kKbBits + 5));
+            n += __popc(bal);
+          }
+          at = wend;
+        } else {
+          const int end = min(at + kSeg, hi);
+          for (int i0 = at; i0 < end; i0 += 32) {
+            const int i = i0 + lane;
+            int kb = i;
+            bool good = i < end;
+            if (sh.mode == 1) {
+              kb = good ? idx[0][i] : INT32_MAX;
+              int before = __shfl_up_sync(0xffffffffu, kb, 1);
+              if (lane == 0) before = prev[0];
+              prev[0] = __shfl_sync(0xffffffffu, kb, min(31, end - 1 - i0));
+              if (good && kb < 0) {
+                set_err(a.err, TASFT_DEVERR_INDEX);
+                good = false;
+              } else if (good && kb <= before) {
+                set_err(a.err, TASFT_DEVERR_ORDER);
+                good = false;
+              }
+              if (kb > qb[0]) good = false;
+            }
+            const unsigned bal = __ballot_sync(0xffffffffu, good);
+            if (good) list[n + __popc(bal & ((1u << lane) - 1u))] = kb | (1 << (kKbBits + 4));
+            n += __popc(bal);
+          }
+          at = end;
+        }
+        __syncwarp();
+        // ---- their pages ----
+        for (int i = lane; i < n; i += 32) {
+          const int e = list[i], kb = e & kKbMask;
+          int pg[4] = {0, 0, 0, 0}, have = 0;
+          const int32_t* row = a.block_table + (int64_t)b * a.max_pages;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (x >= geo.nsub) break;
+            const int tok = kb * kChunkBlk + x * geo.sub_rows;
+            if (tok < w.len) {  // kv_len is within the table's capacity
+              const int p = row[tok / a.page_size];
+              if (p >= 0 && p < a.num_pages) {
+                pg[x] = p;
+                have |= 1 << x;
+              } else {
+                set_err(a.err, TASFT_DEVERR_INDEX);
+              }
+            }
+          }
+          list[i] = e | (have << kKbBits);
+          pgs[i] = make_int4(pg[0], pg[1], pg[2], pg[3]);
+        }
+        __syncwarp();
+        const bool last = at >= hi;
+        if (sh.mode == 2 && n == 0 && !last) continue;  // an empty window: the next one
+        if (lane == 0) {
+          w.n = n;
+          w.first = first;
+          w.last = last;
+          works[lb] = w;
+          mbar_arrive(&list_full[lb]);  // release: the entries, their pages and the record
+        }
+        first = false;
+        ++u;
+        if (last) break;
+      }
+      if (done) break;
+    }
+  } else if (warp == 0) {
+    // ================= producer =================
+    if (lane == 0) {
+      tc::prefetch_tmap(&tmq);
+      tc::prefetch_tmap(&tmk);
+      tc::prefetch_tmap(&tmv);
+      const int nsub = max(1, kChunkBlk / a.page_size), sub_rows = min(kChunkBlk, a.page_size);
+      const uint32_t q_bytes = sh.mode == 2 ? 0 : (uint32_t)(L::kChunks * sh.hpt * sh.tpt * 128);
+      int gk = 0, tile = 0;
+      bool ok = true;
+      for (int u = 0; ok; ++u) {
+        const int lb = u & 1;
+        if (!mbar_wait(&list_full[lb], (u >> 1) & 1)) { ok = false; break; }
+        const Work& w = works[lb];
+        const int n = w.n;
+        if (n < 0) break;
+        if (w.first) {
+          if (tile >= 1 && !mbar_wait(q_empty, (tile - 1) & 1)) { ok = false; break; }
+          if (sh.mode == 2) {
+            const int nv = (w.valid[0] ? 1 : 0) + (w.valid[1] ? 1 : 0);
+            mbar_arrive_expect_tx(q_full, nv * L::kChunks * 64 * 128);
+            for (int x = 0; x < 2; ++x) {
+              if (!w.valid[x]) continue;
+              for (int c = 0; c < L::kChunks; ++c)
+                tc::tma_load_4d(sQ + c * 128 * 128 + x * 64 * 128, &tmq, c * 64, w.head[x], w.row[x], 0, q_full);
+            }
+          } else {
+            mbar_arrive_expect_tx(q_full, q_bytes);
+            for (int c = 0; c < L::kChunks; ++c)
+              tc::tma_load_4d(sQ + c * 128 * 128, &tmq, c * 64, w.head[0], w.row[0], 0, q_full);
+          }
+          ++tile;
+        }
+        const int32_t* list = lists + lb * kSeg;
+        const int32_t* pgs = reinterpret_cast<const int32_t*>(pages + lb * kSeg);
+        // one entry's K or V: the share of each page it has, into the stage's rows
+        auto load = [&](int gi, int j, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off) -> bool {
+          const int st = gi & 1;
+          if (gi >= 2 && !mbar_wait(&empty[st], ((gi >> 1) - 1) & 1)) return false;
+          const int e = list[j], have = (e >> kKbBits) & 15;
+          const int in_page = a.page_size > kChunkBlk ? ((e & kKbMask) & 1) * kChunkBlk : 0;
+          uint8_t* dst = smem + L::kStageOff + off + st * L::kKVTileBytes;
+          mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * L::kChunks * sub_rows * 128));
+          for (int x = 0; x < nsub; ++x) {
+            if (!((have >> x) & 1)) continue;
+            for (int c = 0; c < L::kChunks; ++c)
+              tc::tma_load_4d(dst + c * 64 * 128 + x * sub_rows * 128, map, c * 64, w.hk, in_page, pgs[4 * j + x],
+                              &full[st]);
+          }
+          return true;
+        };
+        // K(j) then V(j-1): the order the MMA warp consumes them
+        for (int j = 0; ok && j <= n && n > 0; ++j) {
+          if (j < n && !load(gk + j, j, &tmk, k_full, k_empty, L::kKOff)) ok = false;
+          if (ok && j >= 1 && !load(gk + j - 1, j - 1, &tmv, v_full, v_empty, L::kVOff)) ok = false;
+        }
+        gk += n;
+      }
+      if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 10));
+      // do not leave while copies into shared memory are in flight
+      if (tile > 0) mbar_wait(q_full, (tile - 1) & 1);
+      for (int i = max(0, gk - 2); ok && i < gk; ++i) {
+        mbar_wait(&k_full[i & 1], (i >> 1) & 1);
+        mbar_wait(&v_full[i & 1], (i >> 1) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ================= MMA issuer =================
+    if (lane == 0) {
+      constexpr uint32_t fmt = kF16 ? 0u : 1u;
+      constexpr uint32_t idesc_s = tc::make_idesc(128, 64, fmt, false);
+      constexpr uint32_t idesc_o = tc::make_idesc(128, D, fmt, true);
+      const uint32_t q_addr = smem_u32(sQ);
+      int g = 0, tile = -1;
+      bool ok = true, started = false;
+      auto issue_s = [&](int gi) -> bool {
+        const int st = gi & 1;
+        if (!mbar_wait(&k_full[st], (gi >> 1) & 1)) return false;
+        // S(gi) overwrites P(gi - 2) in TMEM: P.V(gi - 2) was issued earlier by this thread, and
+        // the MMAs of one thread run through the tensor pipe in issue order
+        tc::tc_fence_after();
+        const uint32_t k_addr = smem_u32(smem + L::kStageOff + L::kKOff + st * L::kKVTileBytes);
+        const uint32_t dst = tS0 + st * 64;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t ad = tc::make_sdesc(q_addr + (kk >> 2) * 128 * 128 + (kk & 3) * 32, 16, 1024);
+          const uint64_t bd = tc::make_sdesc(k_addr + (kk >> 2) * 64 * 128 + (kk & 3) * 32, 16, 1024);
+          tc::mma_ss(dst, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        tc::mma_commit(&s_full[st]);
+        tc::mma_commit(&k_empty[st]);
+        return true;
+      };
+      for (int u = 0; ok; ++u) {
+        const int lb = u & 1;
+        if (!mbar_wait(&list_full[lb], (u >> 1) & 1)) { ok = false; break; }
+        const int n = works[lb].n, first = works[lb].first, last = works[lb].last;
+        if (n < 0) break;
+        if (first) {
+          ++tile;
+          started = false;
+          if (!mbar_wait(q_full, tile & 1)) { ok = false; break; }
+          tc::tc_fence_after();
+        }
+        if (n > 0) ok = issue_s(g);
+        if (ok && last && n <= 1) tc::mma_commit(q_empty);  // no further S of this tile reads Q
+        for (int j = 0; ok && j < n; ++j) {
+          const int gi = g + j;
+          if (j + 1 < n) {
+            ok = issue_s(gi + 1);
+            if (!ok) break;
+            if (last && j + 2 == n) tc::mma_commit(q_empty);
+          }
+          if (!mbar_wait(&p_ready[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
+          // O is reused: the previous tile's epilogue must have read it
+          if (!started && tile >= 1 && !mbar_wait(o_free, (tile - 1) & 1)) { ok = false; break; }
+          if (!mbar_wait(&v_full[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
+          tc::tc_fence_after();
+          const uint32_t v_addr = smem_u32(smem + L::kStageOff + L::kVOff + (gi & 1) * L::kKVTileBytes);
+          const uint32_t p_tmem = tS0 + (gi & 1) * 64;
+#pragma unroll
+          for (int kk = 0; kk < kChunkBlk / 16; ++kk) {
+            const uint64_t bd = tc::make_sdesc(v_addr + kk * 16 * 128, 64 * 128, 1024);
+            tc::mma_ts(tO, p_tmem + kk * 8, bd, idesc_o, (started || kk > 0) ? 1u : 0u);
+          }
+          started = true;
+          tc::mma_commit(&v_empty[gi & 1]);
+          tc::mma_commit(&pv_done[gi & 1]);
+        }
+        if (!ok) break;
+        if (last) {
+          if (!started && tile >= 1 && !mbar_wait(o_free, (tile - 1) & 1)) { ok = false; break; }
+          tc::mma_commit(o_final);
+        }
+        g += n;
+      }
+      if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 11));
+    }
+  } else if (warp >= 4) {
+    // ================= softmax + epilogue (warps 4..7) =================
+    const int quarter = warp & 3;       // TMEM lanes [32*quarter, 32*quarter + 32)
+    const int r = quarter * 32 + lane;  // tile row
+    const int slot = sh.mode == 2 ? r >> 6 : 0;
+    const int tok = sh.mode == 2 ? r & 63 : r / sh.hpt;   // token of the row within its slot
+    const int hd = sh.mode == 2 ? 0 : r % sh.hpt;
+    const int sub_rows = min(kChunkBlk, a.page_size);
+    const int all_pages = (1 << max(1, kChunkBlk / a.page_size)) - 1;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const float sl2 = a.scale * kLog2e;
+    using T = typename std::conditional<kF16, __half, __nv_bfloat16>::type;
+    int g = 0, tile = -1;
+    bool ok = true, started = false;
+    float m = -INFINITY, l = 0.f;
+    for (int u = 0; ok; ++u) {
+      const int lb = u & 1;
+      if (!warp_wait(&list_full[lb], (u >> 1) & 1)) { ok = false; break; }
+      const Work* w = &works[lb];
+      const int n = w->n, last = w->last, len = w->len;
+      if (n < 0) break;
+      const int32_t* list = lists + lb * kSeg;
+      const int qpos = w->pos[slot] + tok;
+      const bool live = sh.mode == 2 ? w->valid[slot] && qpos >= w->ctx && qpos < len : tok < w->valid[0];
+      if (w->first) {
+        ++tile;
+        started = false;
+        m = -INFINITY;
+        l = 0.f;
+      }
+      for (int j = 0; j < n; ++j) {
+        const int gi = g + j;
+        if (!warp_wait(&s_full[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
+        tc::tc_fence_after();
+        const int entry = list[j];
+        const int kbase = (entry & kKbMask) * kChunkBlk;
+        const int have = (entry >> kKbBits) & 15;
+        uint32_t sraw[64];
+        tc::tmem_ld64_sync(tS0 + (gi & 1) * 64 + lane_off, sraw);
+        // keys this row may see: up to its own position
+        int lim = qpos - kbase + 1;
+        if (!live || !((entry >> (kKbBits + 4 + slot)) & 1)) lim = 0;
+        lim = max(0, min(lim, kChunkBlk));
+        float sv[64];
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sv[c] = __uint_as_float(sraw[c]);
+        if (__any_sync(0xffffffffu, lim < kChunkBlk)) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c >= lim) sv[c] = -INFINITY;
+        }
+        if (have != all_pages) {  // keys of a page that is not there
+          uint64_t seen = 0;
+          for (int x = 0; x * sub_rows < kChunkBlk; ++x)
+            if ((have >> x) & 1) seen |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (!((seen >> c) & 1)) sv[c] = -INFINITY;
+        }
+        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+          for (int qd = 0; qd < 4; ++qd) mq[qd] = max3(mq[qd], sv[c + 2 * qd], sv[c + 2 * qd + 1]);
+        }
+        const float mb = max3(mq[0], mq[1], fmaxf(mq[2], mq[3]));
+        const float m_new = fmaxf(m, mb * sl2);
+        const bool need = (m != -INFINITY) && (m_new > m + kRescaleThreshold);
+        if (m == -INFINITY) m = m_new;  // O row is still exactly zero: no rescale
+        if (__any_sync(0xffffffffu, need)) {
+          // O must hold every earlier P.V of this tile before it is rescaled
+          if (!warp_wait(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1)) { ok = false; break; }
+          tc::tc_fence_after();
+          const float alpha = need ? ex2(m - m_new) : 1.0f;
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            tc::tmem_ld32_sync(tO + c0 + lane_off, o);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            tc::tmem_st32(tO + c0 + lane_off, o);
+          }
+          tc::tmem_wait_st();
+          if (need) {
+            l *= alpha;
+            m = m_new;
+          }
+        }
+        uint32_t pk[32];
+        float rs = 0.f;
+        if (m == -INFINITY) {  // nothing to see yet, or only scores that are NaN
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pk[c] = 0u;
+          if (lim > 0) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (sv[c] != sv[c]) rs = sv[c];
+          }
+        } else {
+          const uint64_t sc2 = f2(sl2, sl2), nm2 = f2(-m, -m);
+          uint64_t rs2 = 0;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const uint64_t x2 = fma2(f2(sv[2 * c], sv[2 * c + 1]), sc2, nm2);  // s * scale - m
+            const uint64_t p2 = f2(ex2(lo_f(x2)), ex2(hi_f(x2)));
+            rs2 = add2(rs2, p2);
+            pk[c] = kF16 ? tc::pack_f16x2(lo_f(p2), hi_f(p2)) : tc::pack_bf16x2(lo_f(p2), hi_f(p2));
+          }
+          rs = lo_f(rs2) + hi_f(rs2);
+        }
+        l += rs;
+        tc::tmem_st32(tS0 + (gi & 1) * 64 + lane_off, pk);
+        tc::tmem_wait_st();
+        if (have != all_pages || kbase + kChunkBlk > len) {
+          // rows of V that stand for no key are zeroed (V(gi + 2) cannot land before this
+          // block's P.V, which waits for these threads: the wait below is at most a phase behind)
+          if (!warp_wait(&v_full[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
+          uint8_t* vt = smem + L::kStageOff + L::kVOff + (gi & 1) * L::kKVTileBytes;
+          for (int i = r; i < 64 * L::kChunks * 8; i += 128) {  // 16-byte pieces
+            const int vr = (i >> 3) & 63;
+            if (kbase + vr >= len || !((have >> (vr / sub_rows)) & 1))
+              reinterpret_cast<uint4*>(vt)[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        tc::tc_fence_before();
+        mbar_arrive(&p_ready[gi & 1]);
+        started = true;
+      }
+      if (!ok) break;
+      g += n;
+      if (last) {
+        if (!warp_wait(o_final, tile & 1)) { ok = false; break; }
+        tc::tc_fence_after();
+        const bool direct = w->part < 0;
+        if (direct) {
+          T* orow = reinterpret_cast<T*>(a.out) + (int64_t)(w->row[slot] + tok) * a.o_stride[0] +
+                    (int64_t)(w->head[slot] + hd) * a.o_stride[1];
+          const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that kept nothing gives 0
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            if (started) {
+              tc::tmem_ld32_sync(tO + c0 + lane_off, o);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) o[c] = 0u;
+            }
+            if (live) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float v0 = __uint_as_float(o[2 * c]) * inv;
+                const float v1 = __uint_as_float(o[2 * c + 1]) * inv;
+                pk[c] = kF16 ? tc::pack_f16x2(v0, v1) : tc::pack_bf16x2(v0, v1);
+              }
+              uint4* dst = reinterpret_cast<uint4*>(orow + c0);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) dst[v] = make_uint4(pk[4 * v], pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+            }
+          }
+        } else {
+          const int64_t prow = (int64_t)w->part * sh.rows + r;
+          if (live) ws.ml[prow] = make_float2(m, l);
+          if (started) {
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t o[32];
+              tc::tmem_ld32_sync(tO + c0 + lane_off, o);
+              if (live) {
+                float4* dst = reinterpret_cast<float4*>(ws.o + prow * D + c0);
+#pragma unroll
+                for (int v = 0; v < 8; ++v)
+                  dst[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                                       __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
+              }
+            }
+          }
+        }
+        tc::tc_fence_before();
+        mbar_arrive(o_free);
+      }
+      mbar_arrive(&list_empty[lb]);
+    }
+    if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 12));
+  }
+  // ---------------- teardown ----------------
+  __syncwarp();
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Rows of split items: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, splits in order.
+// One warp per (token, query head); D / 32 consecutive columns per lane.
+template <int D, bool kF16>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const tasft_chunk_args a, const ChunkShape sh, const ChunkWs ws) {
+  using T = typename std::conditional<kF16, __half, __nv_bfloat16>::type;
+  constexpr int V = D / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int grp = a.Hq / a.Hk;
+  const int64_t rows = (int64_t)a.T * a.Hq;
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < rows;
+       i += (int64_t)gridDim.x * (blockDim.x >> 5)) {
+    const int t = (int)(i / a.Hq), head = (int)(i % a.Hq);
+    int bl = 0, bh = a.B - 1;
+    while (bl < bh) {  // last sequence that starts at or before the token (empty ones share a start)
+      const int mid = (bl + bh + 1) >> 1;
+      if (a.cu_seqlens[mid] <= t) bl = mid;
+      else bh = mid - 1;
+    }
+    const ChunkSeq s = chunk_seq(a, sh, bl);
+    if (s.n == 0 || t < s.start || t >= s.start + s.n) continue;
+    const int2 plan = ws.plan[bl];
+    const int ns = plan.x;
+    if (ns <= 1) continue;
+    const int pos = s.ctx + t - s.start, hk = head / grp, hg = head % grp;
+    int tile, unit, row;
+    if (sh.mode == 2) {
+      tile = pos / sh.tpt - s.ctx / sh.tpt;
+      unit = grp >= 2 ? hk * ((grp + 1) / 2) + hg / 2 : hk;
+      row = grp >= 2 ? (hg & 1) * 64 + (pos & 63) : pos & 127;
+    } else {
+      unit = hk;
+      if (sh.mode == 0) {
+        tile = (t - s.start) / sh.tpt;
+        row = (t - s.start - tile * sh.tpt) * sh.hpt + hg;
+      } else {
+        tile = pos / sh.tpt - s.ctx / sh.tpt;
+        row = (pos - max(s.ctx, (pos / sh.tpt) * sh.tpt)) * sh.hpt + hg;
+      }
+    }
+    const int64_t part = plan.y + (int64_t)(tile * sh.units + unit) * ns;
+    float M = -INFINITY;
+    for (int x = lane; x < ns; x += 32) M = fmaxf(M, ws.ml[(part + x) * sh.rows + row].x);
+    M = warp_max(M);
+    float acc[V], sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc[c] = 0.f;
+#pragma unroll 4
+    for (int x = 0; x < ns; ++x) {
+      const int64_t pr = (part + x) * sh.rows + row;
+      const float2 ml = ws.ml[pr];
+      if (ml.y == 0.f) continue;  // a slice with nothing to see wrote no O
+      const float wgt = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
+      sum += wgt * ml.y;
+      const float* o = ws.o + pr * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(o);
+        acc[0] += wgt * v.x; acc[1] += wgt * v.y; acc[2] += wgt * v.z; acc[3] += wgt * v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(o);
+        acc[0] += wgt * v.x; acc[1] += wgt * v.y;
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* orow = reinterpret_cast<T*>(a.out) + (int64_t)t * a.o_stride[0] + (int64_t)head * a.o_stride[1] + lane * V;
+    uint32_t pk[V / 2];
+#pragma unroll
+    for (int c = 0; c < V / 2; ++c)
+      pk[c] = kF16 ? tc::pack_f16x2(acc[2 * c] * inv, acc[2 * c + 1] * inv)
+                   : tc::pack_bf16x2(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(orow) = make_uint2(pk[0], pk[1]);
+    else *reinterpret_cast<uint32_t*>(orow) = pk[0];
+  }
+}
+
+// How a call's tiles are laid out; false when no layout covers it.
+bool chunk_shape(ChunkShape& sh, int Hq, int Hk, int Hm, int max_q) {
+  const int grp = Hq / Hk;
+  if (grp > 64) return false;
+  if (Hm > 0 && (Hm != Hk || grp == 1)) {
+    sh.mode = 2;
+    sh.hpt = 1;
+    sh.tpt = grp >= 2 ? 64 : 128;
+    sh.units = grp >= 2 ? Hk * ((grp + 1) / 2) : Hk;
+    sh.rows = 128;
+  } else {
+    sh.mode = Hm > 0 ? 1 : 0;
+    sh.hpt = grp;
+    sh.units = Hk;
+    sh.tpt = 128 / grp;
+    if (sh.mode == 1) {
+      int t = 64;
+      while (t > sh.tpt) t >>= 1;
+      sh.tpt = t;
+    }
+    sh.rows = grp * (max_q < sh.tpt ? max_q : sh.tpt);
+  }
+  return true;
+}
+
+int64_t plan_bytes(int B) { return ((int64_t)B * 8 + 255) / 256 * 256; }
+int64_t slot_bytes(const ChunkShape& sh, int D) { return (int64_t)sh.rows * (D + 2) * 4; }
+
+template <int D, bool kF16>
+int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  const int box = a.page_size < kChunkBlk ? a.page_size : kChunkBlk;
+  if (!make_tmap_thd(&mq, a.q, a.T, a.Hq, D, a.q_stride[0], a.q_stride[1], sh.mode == 2 ? 1 : sh.hpt,
+                     sh.mode == 2 ? 64 : sh.tpt))
+    return TASFT_ERR_UNSUPPORTED;
+  if (!make_tmap_paged(&mk, a.k_pages, a.num_pages, a.page_size, a.Hk, D, a.k_stride, box)) return TASFT_ERR_UNSUPPORTED;
+  if (!make_tmap_paged(&mv, a.v_pages, a.num_pages, a.page_size, a.Hk, D, a.v_stride, box)) return TASFT_ERR_UNSUPPORTED;
+  auto kern = bsa_chunk_tc_kernel<D, kF16>;
+  const int smem = Smem<D>::kAlloc;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return TASFT_ERR_CUDA;
+  ChunkWs ws;
+  uint8_t* p = reinterpret_cast<uint8_t*>(a.workspace);
+  ws.plan = reinterpret_cast<int2*>(p);
+  ws.ml = reinterpret_cast<float2*>(p + plan_bytes(a.B));
+  ws.o = reinterpret_cast<float*>(p + plan_bytes(a.B) + ((int64_t)sh.slots * sh.rows * 8 + 255) / 256 * 256);
+  const int grid = 2 * sms;  // persistent: two CTAs per SM
+  if (debug_enabled()) debug_log("chunk_tc D=%d mode=%d grid=%d slots=%d smem=%d", D, sh.mode, grid, sh.slots, smem);
+  kern<<<grid, kThreads, smem, st>>>(mq, mk, mv, a, sh, ws);
+  count_launch();
+  int rc = launch_status();
+  if (rc != TASFT_OK || sh.slots == 0) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)sms * 2);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  rc = cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<D, kF16>, a, sh, ws));
+  count_launch();
+  return rc;
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();  // no device: the size query still answers
+    return 148;
+  }
+  return sms;
+}
+
+}  // namespace
+}  // namespace tasft
+
+using namespace tasft;
+
+extern "C" int64_t tasft_chunk_workspace_size(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q,
+                                              int32_t Hm) {
+  if (B <= 0 || T < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D <= 0 || max_q <= 0 || Hm < 0) return TASFT_ERR_INVALID_ARG;
+  ChunkShape sh;
+  if (!chunk_shape(sh, Hq, Hk, Hm, max_q)) return TASFT_ERR_UNSUPPORTED;
+  // Pieces hold at least a CTA's mean load, so split tiles make at most twice as many pieces as
+  // there are CTAs; and a tile makes at most kChunkMaxSplits.
+  const int64_t tiles = ((int64_t)T / sh.tpt + 2LL * B) * sh.units;
+  int64_t slots = 4LL * sm_count();
+  if (tiles * kChunkMaxSplits < slots) slots = tiles * kChunkMaxSplits;
+  return plan_bytes(B) + slots * slot_bytes(sh, D) + 256;
+}
+
+extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_stream_t stream) {
+  if (!ap) return TASFT_ERR_INVALID_ARG;
+  const tasft_chunk_args& a = *ap;
+  if (a.B <= 0 || a.T < 0 || a.Hq <= 0 || a.Hk <= 0 || a.D <= 0 || a.Hq % a.Hk != 0 || a.max_q <= 0 ||
+      a.max_pages <= 0 || a.num_pages <= 0 || !(a.scale > 0.f))
+    return TASFT_ERR_INVALID_ARG;
+  if (!a.cu_seqlens || !a.kv_len || !a.block_table || !a.k_pages || !a.v_pages) return TASFT_ERR_INVALID_ARG;
+  if (a.k_stride[3] != 1 || a.v_stride[3] != 1) return TASFT_ERR_INVALID_ARG;
+  if (a.kept_idx) {
+    if (!a.kept_cnt || (a.Hm != a.Hk && a.Hm != a.Hq) || a.nb_w <= 0 || a.nb_q < (a.max_q + 126) / 64)
+      return TASFT_ERR_INVALID_ARG;
+  }
+  if (a.T == 0) return TASFT_OK;
+  if (!a.q || !a.out) return TASFT_ERR_INVALID_ARG;
+  if (a.dtype != TASFT_BF16 && a.dtype != TASFT_F16) return TASFT_ERR_UNSUPPORTED;
+  if ((a.D != 64 && a.D != 128) || a.block != kChunkBlk) return TASFT_ERR_UNSUPPORTED;
+  if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size != 128) return TASFT_ERR_UNSUPPORTED;
+  // block indices travel in kKbBits bits
+  if ((int64_t)a.max_pages * a.page_size > (int64_t)kKbMask * kChunkBlk) return TASFT_ERR_TOO_LARGE;
+  // 16-byte stores of out's rows (q and the pages are checked with their tensor maps)
+  if (!aligned16(a.out) || a.o_stride[0] % 8 || a.o_stride[1] % 8) return TASFT_ERR_UNSUPPORTED;
+  ChunkShape sh;
+  if (!chunk_shape(sh, a.Hq, a.Hk, a.kept_idx ? a.Hm : 0, a.max_q)) return TASFT_ERR_UNSUPPORTED;
+  sh.capacity = a.max_pages * a.page_size;
+  const int blocks = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
+  sh.bound = a.kept_idx && a.nb_w * (sh.mode == 2 ? 2 : 1) < blocks ? a.nb_w * (sh.mode == 2 ? 2 : 1) : blocks;
+  sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
+  if (!a.workspace || a.workspace_bytes < plan_bytes(a.B)) return TASFT_ERR_WORKSPACE;
+  const int64_t slots = (a.workspace_bytes - plan_bytes(a.B) - 256) / slot_bytes(sh, a.D);
+  sh.slots = (int)(slots < 0 ? 0 : slots > (1 << 20) ? (1 << 20) : slots);
+  if (sh.bound <= kChunkMinPiece) sh.slots = 0;  // nothing that long: one launch
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int sms = sm_count();
+  const bool f16 = a.dtype == TASFT_F16;
+  if (a.D == 128) return f16 ? launch<128, true>(a, sh, sms, st) : launch<128, false>(a, sh, sms, st);
+  return f16 ? launch<64, true>(a, sh, sms, st) : launch<64, false>(a, sh, sms, st);
+}

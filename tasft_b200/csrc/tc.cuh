@@ -166,6 +166,11 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 bool make_tmap_paged(CUtensorMap* map, const void* base, int pages, int page_size, int H, int D,
                      const int64_t* stride_elems, int box_rows);
 
+// Host: map over packed rows [T, H, D] (element strides of token and head, D contiguous) as dims
+// {D, H, T, 1}; box {64, box_heads, box_tokens, 1}, rows token-major, 128-byte swizzled.
+bool make_tmap_thd(CUtensorMap* map, const void* base, int T, int H, int D, int64_t token_stride, int64_t head_stride,
+                   int box_heads, int box_tokens);
+
 bool make_tmap_bhsd(CUtensorMap* map, const void* base, int B, int H, int S, int D, const int64_t* stride_elems,
                     int elem_bytes, int box_rows);
 

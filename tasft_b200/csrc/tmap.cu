@@ -61,4 +61,21 @@ bool make_tmap_paged(CUtensorMap* map, const void* base, int pages, int page_siz
   return r == CUDA_SUCCESS;
 }
 
+bool make_tmap_thd(CUtensorMap* map, const void* base, int T, int H, int D, int64_t token_stride, int64_t head_stride,
+                   int box_heads, int box_tokens) {
+  auto fn = get_encode();
+  if (!fn) return false;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || D % 64 != 0) return false;
+  if (token_stride <= 0 || head_stride <= 0 || token_stride % 8 || head_stride % 8) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T, 1};
+  cuuint64_t strides[3] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2, (cuuint64_t)token_stride * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS && debug_enabled()) debug_log("cuTensorMapEncodeTiled (packed) failed: %d", (int)r);
+  return r == CUDA_SUCCESS;
+}
+
 }  // namespace tasft
