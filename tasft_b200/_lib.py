@@ -8,6 +8,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -302,14 +303,28 @@ def strides3(t: torch.Tensor):
 
 
 def stream_ptr(device: torch.device) -> int:
+    if device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)  # the handle without a Stream object (2 us)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def packed(cls):
+    """A constructor of ``cls`` from its fields' plain values in order, arrays flattened and null
+    pointers as 0: one struct.pack, a third of the time that ctypes takes field by field."""
+    codes = {vp: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f", C.c_double: "d"}
+    fmt = "".join(f"{t._length_}{codes[t._type_]}" if hasattr(t, "_length_") else codes[t] for _, t in cls._fields_)
+    pack = struct.Struct("@" + fmt)
+    assert pack.size <= C.sizeof(cls) < pack.size + 8  # the tail padding is the struct's own
+    pad = bytes(C.sizeof(cls) - pack.size)
+    return lambda *values: cls.from_buffer_copy(pack.pack(*values) + pad)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(t: torch.Tensor):
     """Context in which t's device is the current one (launches go to the current device)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def require_cuda(*ts: torch.Tensor) -> None:

@@ -97,45 +97,38 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: dict | None =
     return (f if device is None else f.to(device)), attention
 
 
-def _batch(name: str, device, block_table, cu_seqlens, kv_len):
-    """The batch's int32 index tensors on the tensors' device, contiguous."""
-    B = kv_len.shape[0] if kv_len.ndim == 1 else -1
-    if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] != B + 1 or B <= 0 or (
-            block_table is not None and (block_table.ndim != 2 or block_table.shape[0] != B)):
-        raise KernelError(f"{name}: expects cu_seqlens [B + 1], kv_len [B] and block_table [B, max_pages]",
-                          context={"cu_seqlens": list(cu_seqlens.shape), "kv_len": list(kv_len.shape),
-                                   "table": None if block_table is None else list(block_table.shape)})
-    out = []
-    for t in (block_table, cu_seqlens, kv_len):
-        if t is not None:
-            if t.device != device:
-                raise KernelError(f"{name}: tensors on different devices",
-                                  context={"device": str(device), "got": str(t.device)})
-            if t.dtype != torch.int32:
-                t = t.to(torch.int32)
-            if not t.is_contiguous():
-                t = t.contiguous()
-        out.append(t)
-    return B, *out
+_rope_args = L.packed(L.RopeAppendArgs)
+_select_args = L.packed(L.SelectArgs)
+_chunk_args = L.packed(L.ChunkArgs)
 
 
-def _check_pages(name: str, q, k_pages, v_pages) -> None:
-    if q.ndim != 3 or k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != q.shape[2] \
-            or k_pages.shape[2] == 0 or q.shape[1] == 0 or q.shape[1] % k_pages.shape[2]:
+def _index(name: str, t: torch.Tensor, gpu: int, n: int, ndim: int = 1) -> torch.Tensor:
+    """An index tensor ``[n]`` (``[n, any]``) on the batch's device as contiguous int32."""
+    if t.get_device() != gpu or t.dim() != ndim or t.size(0) != n:
+        raise KernelError(f"{name}: expects cu_seqlens [B + 1], kv_len [B] and block_table [B, max_pages] on one device",
+                          context={"shape": list(t.shape), "rows": n, "device": str(t.device)})
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _check_pages(name: str, gpu: int, q, qs, k_pages, ks, v_pages) -> None:
+    if len(qs) != 3 or len(ks) != 4 or ks != v_pages.shape or ks[3] != qs[2] or not ks[2] or not qs[1] or qs[1] % ks[2]:
         raise KernelError(f"{name}: expects q [T, Hq, D] and pages [num_pages, page_size, Hk, D], Hq a multiple of Hk",
-                          context={"q": list(q.shape), "k_pages": list(k_pages.shape), "v_pages": list(v_pages.shape)})
-    if k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+                          context={"q": list(qs), "k_pages": list(ks), "v_pages": list(v_pages.shape)})
+    if k_pages.dtype is not q.dtype or v_pages.dtype is not q.dtype:
         raise KernelError(f"{name}: q and the pages must have one dtype",
                           context={"q": str(q.dtype), "k": str(k_pages.dtype), "v": str(v_pages.dtype)})
-    if k_pages.device != q.device or v_pages.device != q.device:
-        raise KernelError(f"{name}: tensors on different devices",
+    if gpu < 0 or k_pages.get_device() != gpu or v_pages.get_device() != gpu:
+        raise KernelError(f"{name}: tensors must be on one CUDA device",
                           context={"q": str(q.device), "k": str(k_pages.device), "v": str(v_pages.device)})
 
 
-def _check_err(name: str, device, err) -> None:
-    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != device):
+def _err_ptr(name: str, gpu: int, err) -> int:
+    if err is None:
+        return 0
+    if err.dtype is not torch.int32 or err.numel() < 1 or err.get_device() != gpu:
         raise KernelError(f"{name}: err must be an int32 tensor on the same device",
                           context={"dtype": str(err.dtype), "device": str(err.device)})
+    return err.data_ptr()
 
 
 def rope_append_paged(
@@ -170,49 +163,66 @@ def rope_append_paged(
     :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
     256. The packed, paged counterpart of :func:`qkv_rope_pool`, which takes cos and sin as tables."""
     name = "rope_append_paged"
-    L.require_cuda(q, k, v, inv_freq, k_pages, v_pages, block_table, cu_seqlens, kv_len)
-    _check_pages(name, q, k_pages, v_pages)
-    T, Hq, D = q.shape
-    num_pages, page_size, Hk, _ = k_pages.shape
-    if k.shape != (T, Hk, D) or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise KernelError(f"{name}: expects k, v [T, Hk, D] in q's dtype",
-                          context={"q": list(q.shape), "k": list(k.shape), "v": list(v.shape)})
+    gpu, qs, ks = q.get_device(), q.shape, k_pages.shape
+    _check_pages(name, gpu, q, qs, k_pages, ks, v_pages)
+    T, Hq, D = qs
+    num_pages, page_size, Hk, _ = ks
+    dtype = q.dtype
+    if k.shape != (T, Hk, D) or v.shape != (T, Hk, D) or k.dtype is not dtype or v.dtype is not dtype or \
+            k.get_device() != gpu or v.get_device() != gpu:
+        raise KernelError(f"{name}: expects k, v [T, Hk, D] in q's dtype and on its device",
+                          context={"q": list(qs), "k": list(k.shape), "v": list(v.shape)})
     if block != BLOCK or max_new <= 0:
         raise KernelError(f"{name}: block must be {BLOCK}, max_new positive",
                           context={"block": block, "max_new": max_new})
-    if inv_freq.ndim != 1 or inv_freq.dtype not in (torch.float64, torch.float32):
-        raise KernelError(f"{name}: inv_freq must be [rot / 2], fp64 or fp32",
+    f64 = inv_freq.dtype is torch.float64
+    if inv_freq.dim() != 1 or not (f64 or inv_freq.dtype is torch.float32) or inv_freq.get_device() != gpu:
+        raise KernelError(f"{name}: inv_freq must be [rot / 2], fp64 or fp32, on the same device",
                           context={"shape": list(inv_freq.shape), "dtype": str(inv_freq.dtype)})
     dev = q.device
-    B, table, cu, kvl = _batch(name, dev, block_table, cu_seqlens, kv_len)
-    _check_err(name, dev, err)
+    B = kv_len.numel()
+    kvl = _index(name, kv_len, gpu, B)
+    cu = _index(name, cu_seqlens, gpu, B + 1)
+    table = _index(name, block_table, gpu, B, 2)
+    err_ptr = _err_ptr(name, gpu, err)
     rows = chunk_rows(max_new)
-    nbk = 0
+    nbk = pq_ptr = pk_ptr = 0
     pooled_q = None
     if pooled_k is not None:
-        if pooled_k.ndim != 4 or pooled_k.dtype != torch.float32 or not pooled_k.is_contiguous() or \
-                pooled_k.device != dev or pooled_k.shape[:2] != (B, Hk) or pooled_k.shape[3] != D:
-            raise KernelError(f"{name}: pooled_k must be contiguous fp32 [B, Hk, NBk, D]",
-                              context={"pooled_k": list(pooled_k.shape), "dtype": str(pooled_k.dtype)})
-        nbk = pooled_k.shape[2]
+        ps = pooled_k.shape
+        if len(ps) != 4 or ps[0] != B or ps[1] != Hk or ps[3] != D or pooled_k.dtype is not torch.float32 or \
+                not pooled_k.is_contiguous() or pooled_k.get_device() != gpu:
+            raise KernelError(f"{name}: pooled_k must be contiguous fp32 [B, Hk, NBk, D] on the same device",
+                              context={"pooled_k": list(ps), "dtype": str(pooled_k.dtype)})
+        nbk = ps[2]
         pooled_q = torch.empty(B, Hq, rows, D, dtype=torch.float32, device=dev)
+        pq_ptr, pk_ptr = pooled_q.data_ptr(), pooled_k.data_ptr()
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
-        raise KernelError(f"{name}: out must match q", context={"q": list(q.shape), "out": list(out.shape)})
-    q, k, v = (x if x.stride(2) == 1 else x.contiguous() for x in (q, k, v))
+        out = torch.empty(T, Hq, D, dtype=dtype, device=dev)
+    elif out.shape != qs or out.dtype is not dtype or out.get_device() != gpu or out.stride(2) != 1:
+        raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
+    (q, qt), (k, kt), (v, vt) = _rows(q), _rows(k), _rows(v)
     freq = inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
     with L.on_device(q):
-        args = L.RopeAppendArgs(
+        args = _rope_args(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            L.I64x2(*q.stride()[:2]), L.I64x2(*k.stride()[:2]), L.I64x2(*v.stride()[:2]), L.I64x2(*out.stride()[:2]),
-            L.strides4(k_pages), L.strides4(v_pages), freq.data_ptr(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(),
-            L.ptr(pooled_q), L.ptr(pooled_k), float(attention_scaling), B, T, Hq, Hk, D, 2 * freq.shape[0], block,
-            L.dtype_code(q), int(max_new), table.shape[1], page_size, num_pages, rows, nbk, int(interleaved),
-            int(freq.dtype == torch.float64), L.ptr(err))
-        L.check(L.lib().tasft_rope_append_paged(args, L.stream_ptr(dev)), "tasft_rope_append_paged",
-                shape=[B, T, Hq, Hk, D], page_size=page_size)
+            qt[0], qt[1], kt[0], kt[1], vt[0], vt[1], out.stride(0), out.stride(1), *k_pages.stride(), *v_pages.stride(),
+            freq.data_ptr(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), pq_ptr, pk_ptr, attention_scaling,
+            B, T, Hq, Hk, D, 2 * freq.numel(), block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, rows,
+            nbk, interleaved, f64, err_ptr)
+        rc = L.lib().tasft_rope_append_paged(args, L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "tasft_rope_append_paged", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out, pooled_q
+
+
+def _rows(x: torch.Tensor):
+    """x with contiguous columns, and its strides."""
+    st = x.stride()
+    if st[2] != 1:
+        x = x.contiguous()
+        st = x.stride()
+    return x, st
 
 
 def select_blocks(
@@ -239,32 +249,34 @@ def select_blocks(
     :func:`bsa_decode_paged` take row 0 (``idx[:, :, 0]``, ``cnt[:, :, 0]``). Beside
     :func:`threshold_scores`, which keeps by threshold alone."""
     name = "select_blocks"
-    L.require_cuda(scores, cu_seqlens, kv_len)
-    if scores.ndim != 4 or scores.dtype != torch.float32 or num_kv_heads <= 0 or scores.shape[1] % num_kv_heads:
-        raise KernelError(f"{name}: expects fp32 scores [B, Hq, NBq, NBk], Hq a multiple of num_kv_heads",
-                          context={"scores": list(scores.shape), "dtype": str(scores.dtype), "Hk": num_kv_heads})
+    gpu, shape = scores.get_device(), scores.shape
+    if len(shape) != 4 or scores.dtype is not torch.float32 or num_kv_heads <= 0 or shape[1] % num_kv_heads or gpu < 0:
+        raise KernelError(f"{name}: expects fp32 scores [B, Hq, NBq, NBk] on a CUDA device, Hq a multiple of num_kv_heads",
+                          context={"scores": list(shape), "dtype": str(scores.dtype), "Hk": num_kv_heads,
+                                   "device": str(scores.device)})
     if top_k <= 0 or first < 0 or local < 1 or block <= 0:
         raise ValidationError(f"{name}: top_k and local must be positive, first not negative",
                               context={"top_k": top_k, "first": first, "local": local, "block": block})
-    dev = scores.device
-    B, _, cu, kvl = _batch(name, dev, None, cu_seqlens, kv_len)
-    if scores.shape[0] != B:
-        raise KernelError(f"{name}: scores and kv_len disagree about the batch",
-                          context={"scores": list(scores.shape), "kv_len": list(kv_len.shape)})
-    _check_err(name, dev, err)
-    if scores.stride(3) != 1:
+    B, Hq, nbq, nbk = shape
+    st = scores.stride()
+    if st[3] != 1:
         scores = scores.contiguous()
-    _, Hq, nbq, nbk = scores.shape
+        st = scores.stride()
+    kvl = _index(name, kv_len, gpu, B)
+    cu = _index(name, cu_seqlens, gpu, B + 1)
+    err_ptr = _err_ptr(name, gpu, err)
     width = min(nbk, max(top_k, first + local))
+    dev = scores.device
     idx = torch.empty(B, num_kv_heads, nbq, width, dtype=torch.int32, device=dev)
     cnt = torch.empty(B, num_kv_heads, nbq, dtype=torch.int32, device=dev)
     with L.on_device(scores):
-        args = L.SelectArgs(
-            scores.data_ptr(), L.I64x3(*scores.stride()[:3]), cu.data_ptr(), kvl.data_ptr(), B, Hq, num_kv_heads, nbq,
-            nbk, block, min(top_k, nbk), min(first, nbk), min(local, nbk), int(tau is not None),
-            0.0 if tau is None else float(tau), width, idx.data_ptr(), cnt.data_ptr(), L.ptr(err))
-        L.check(L.lib().tasft_select_blocks(args, L.stream_ptr(dev)), "tasft_select_blocks",
-                shape=[B, Hq, num_kv_heads, nbq, nbk])
+        args = _select_args(
+            scores.data_ptr(), st[0], st[1], st[2], cu.data_ptr(), kvl.data_ptr(), B, Hq, num_kv_heads, nbq, nbk, block,
+            min(top_k, nbk), min(first, nbk), min(local, nbk), tau is not None, 0.0 if tau is None else tau, width,
+            idx.data_ptr(), cnt.data_ptr(), err_ptr)
+        rc = L.lib().tasft_select_blocks(args, L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "tasft_select_blocks", shape=[B, Hq, num_kv_heads, nbq, nbk])
     return KeptBlocks(idx, cnt)
 
 
@@ -297,50 +309,58 @@ def bsa_chunk_paged(
     spreads as the softmax formula has it. Beside :func:`bsa_decode_paged` (one token per sequence) and
     :meth:`BlockSparseFlashAttention.forward_varlen` (no cache)."""
     name = "bsa_chunk_paged"
-    L.require_cuda(q, k_pages, v_pages, block_table, cu_seqlens, kv_len)
-    _check_pages(name, q, k_pages, v_pages)
-    T, Hq, D = q.shape
-    num_pages, page_size, Hk, _ = k_pages.shape
+    gpu, qs, ks = q.get_device(), q.shape, k_pages.shape
+    _check_pages(name, gpu, q, qs, k_pages, ks, v_pages)
+    T, Hq, D = qs
+    num_pages, page_size, Hk, _ = ks
     dev = q.device
-    B, table, cu, kvl = _batch(name, dev, block_table, cu_seqlens, kv_len)
-    _check_err(name, dev, err)
+    B = kv_len.numel()
+    kvl = _index(name, kv_len, gpu, B)
+    cu = _index(name, cu_seqlens, gpu, B + 1)
+    table = _index(name, block_table, gpu, B, 2)
+    err_ptr = _err_ptr(name, gpu, err)
     if max_new <= 0:
         raise KernelError(f"{name}: max_new must be positive", context={"max_new": max_new})
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    elif not (scale > 0.0 and math.isfinite(scale)):
         raise KernelError(f"{name}: scale must be positive and finite", context={"scale": scale})
-    idx = cnt = None
-    hm = rows = width = 0
+    idx_ptr = cnt_ptr = hm = rows = width = 0
     if kept is not None:
         idx, cnt = kept.idx, kept.cnt
-        if idx.ndim != 4 or idx.shape[0] != B or idx.shape[1] not in (Hq, Hk) or cnt.shape != idx.shape[:3] or \
-                idx.shape[2] < chunk_rows(max_new) or idx.shape[3] == 0 or idx.device != dev or cnt.device != dev:
-            raise KernelError(f"{name}: kept lists must be [B, Hk or Hq, at least {chunk_rows(max_new)}, W]",
-                              context={"idx": list(idx.shape), "cnt": list(cnt.shape)})
-        if idx.dtype != torch.int32 or not idx.is_contiguous():
+        ls = idx.shape
+        if len(ls) != 4 or ls[0] != B or ls[1] not in (Hq, Hk) or cnt.shape != ls[:3] or ls[2] < chunk_rows(max_new) or \
+                not ls[3] or idx.get_device() != gpu or cnt.get_device() != gpu:
+            raise KernelError(f"{name}: kept lists must be [B, Hk or Hq, at least {chunk_rows(max_new)}, W] on one device",
+                              context={"idx": list(ls), "cnt": list(cnt.shape)})
+        if idx.dtype is not torch.int32 or not idx.is_contiguous():
             idx = idx.to(torch.int32).contiguous()
-        if cnt.dtype != torch.int32 or not cnt.is_contiguous():
+        if cnt.dtype is not torch.int32 or not cnt.is_contiguous():
             cnt = cnt.to(torch.int32).contiguous()
-        _, hm, rows, width = idx.shape
+        idx_ptr, cnt_ptr = idx.data_ptr(), cnt.data_ptr()
+        _, hm, rows, width = ls
     if out is None:
         out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
-        raise KernelError(f"{name}: out must match q", context={"q": list(q.shape), "out": list(out.shape)})
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    elif out.shape != qs or out.dtype is not q.dtype or out.get_device() != gpu or out.stride(2) != 1:
+        raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
+    st = q.stride()
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or q.data_ptr() % 16:
         q = q.contiguous()
+        st = q.stride()
     lib = L.lib()
     with L.on_device(q):
         nbytes = lib.tasft_chunk_workspace_size(B, T, Hq, Hk, D, max_new, hm)
         if nbytes < 0:
             L.check(int(nbytes), "tasft_chunk_workspace_size", shape=[B, T, Hq, Hk, D])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        args = L.ChunkArgs(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), L.I64x2(*q.stride()[:2]),
-            L.I64x2(*out.stride()[:2]), L.strides4(k_pages), L.strides4(v_pages), table.data_ptr(), cu.data_ptr(),
-            kvl.data_ptr(), L.ptr(idx), L.ptr(cnt), B, T, Hq, Hk, D, block, L.dtype_code(q), max_new, table.shape[1],
-            page_size, num_pages, hm, rows, width, scale, ws.data_ptr(), nbytes, L.ptr(err))
-        L.check(lib.tasft_bsa_chunk_paged_fwd(args, L.stream_ptr(dev)), "tasft_bsa_chunk_paged_fwd",
-                shape=[B, T, Hq, Hk, D], page_size=page_size)
+        args = _chunk_args(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), st[0], st[1], out.stride(0),
+            out.stride(1), *k_pages.stride(), *v_pages.stride(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), idx_ptr,
+            cnt_ptr, B, T, Hq, Hk, D, block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, hm, rows, width,
+            scale, ws.data_ptr(), nbytes, err_ptr)
+        rc = lib.tasft_bsa_chunk_paged_fwd(args, L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "tasft_bsa_chunk_paged_fwd", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out
 
 

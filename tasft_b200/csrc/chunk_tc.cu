@@ -904,8 +904,8 @@ int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
   if (!make_tmap_paged(&mv, a.v_pages, a.num_pages, a.page_size, a.Hk, D, a.v_stride, box)) return TASFT_ERR_UNSUPPORTED;
   auto kern = bsa_chunk_tc_kernel<D, kF16>;
   const int smem = Smem<D>::kAlloc;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return TASFT_ERR_CUDA;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(kern, smem, allowed)) return TASFT_ERR_CUDA;
   ChunkWs ws;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.workspace);
   ws.plan = reinterpret_cast<int2*>(p);
@@ -931,15 +931,6 @@ int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
   return rc;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();  // no device: the size query still answers
-    return 148;
-  }
-  return sms;
-}
-
 }  // namespace
 }  // namespace tasft
 
@@ -960,7 +951,12 @@ extern "C" int64_t tasft_chunk_workspace_size(int32_t B, int32_t T, int32_t Hq, 
 
 extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_stream_t stream) {
   if (!ap) return TASFT_ERR_INVALID_ARG;
-  const tasft_chunk_args& a = *ap;
+  tasft_chunk_args a = *ap;
+  // strides of axes of length one say nothing
+  if (a.T == 1) a.q_stride[0] = a.o_stride[0] = a.D;
+  if (a.Hq == 1) a.q_stride[1] = a.o_stride[1] = a.D;
+  if (a.Hk == 1) a.k_stride[2] = a.v_stride[2] = a.D;
+  if (a.num_pages == 1) a.k_stride[0] = a.v_stride[0] = a.D;
   if (a.B <= 0 || a.T < 0 || a.Hq <= 0 || a.Hk <= 0 || a.D <= 0 || a.Hq % a.Hk != 0 || a.max_q <= 0 ||
       a.max_pages <= 0 || a.num_pages <= 0 || !(a.scale > 0.f))
     return TASFT_ERR_INVALID_ARG;

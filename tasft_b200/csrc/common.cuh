@@ -148,6 +148,38 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// SM count of the current device (148 where there is none: size queries still answer), looked
+// up once per device.
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory; `done` (one per kernel) remembers the
+// devices where it already may.
+template <typename K>
+inline bool allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
 inline int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

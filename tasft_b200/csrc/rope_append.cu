@@ -250,15 +250,11 @@ template <typename T, bool kMixed>
 int run(const tasft_rope_append_args& a, cudaStream_t st) {
   auto kern = rope_append_kernel<T, kMixed>;
   const int smem = kRopeBlk * a.rot * (int)sizeof(float);  // cos and sin, rot / 2 each
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return TASFT_ERR_CUDA;
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<uint64_t> allowed{0};
+  if (smem > 48 * 1024 && !allow_smem(kern, kRopeBlk * 256 * (int)sizeof(float), allowed)) return TASFT_ERR_CUDA;
   // shares of the heads: a warp's worth at least, more while CTAs are few
   const int heads = a.Hq + 2 * a.Hk;
-  int64_t z = (4LL * sms + (int64_t)a.B * a.NBq - 1) / ((int64_t)a.B * a.NBq);
+  int64_t z = (4LL * sm_count() + (int64_t)a.B * a.NBq - 1) / ((int64_t)a.B * a.NBq);
   const int most = (heads + 7) / 8;
   if (z > most) z = most;
   if (a.B > 65535) return TASFT_ERR_TOO_LARGE;
@@ -281,7 +277,13 @@ using namespace tasft;
 
 extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_stream_t stream) {
   if (!ap) return TASFT_ERR_INVALID_ARG;
-  const tasft_rope_append_args& a = *ap;
+  tasft_rope_append_args a = *ap;
+  // strides of axes of length one say nothing
+  if (a.T == 1) a.q_stride[0] = a.k_in_stride[0] = a.v_in_stride[0] = a.o_stride[0] = 0;
+  if (a.Hq == 1) a.q_stride[1] = a.o_stride[1] = 0;
+  if (a.Hk == 1) a.k_in_stride[1] = a.v_in_stride[1] = a.k_stride[2] = a.v_stride[2] = 0;
+  if (a.num_pages == 1) a.k_stride[0] = a.v_stride[0] = 0;
+  if (a.page_size == 1) a.k_stride[1] = a.v_stride[1] = 0;
   if (a.B <= 0 || a.T < 0 || a.Hq <= 0 || a.Hk <= 0 || a.Hq % a.Hk || a.D <= 0 || a.max_q <= 0 || a.max_pages <= 0 ||
       a.num_pages <= 0 || a.page_size <= 0)
     return TASFT_ERR_INVALID_ARG;

@@ -3,13 +3,16 @@
 //
 // A block's score is the highest of its group's query heads (NaN counts as -inf; a -inf score
 // is never chosen), optionally with a floor tau. Ties go to the lowest index. The k-th largest
-// score is found exactly, without a sort: scores are mapped to integers of the same order and
-// the threshold's bits are fixed from the top, one count of "at least this much" per bit, over
-// values that stay in registers. Kept blocks become one bit each, and a scan over the words'
-// population counts places them.
+// score is found exactly, without a sort: scores are mapped to integers of the same order, held
+// in registers, and the threshold is fixed from the top. Up to 128 blocks a warp takes a row and
+// counts "at least this much" bit by bit; longer rows take one CTA and eight bits at a time,
+// with a histogram in shared memory, below the bits that the row's largest and smallest score
+// share (gate scores lie close together). Either stops as soon as the count comes out exactly.
+// Kept blocks become one bit each, and a scan over the words' population counts places them.
 //
-// One group of kT threads per row, kV values per thread (value i of thread t is block
-// i * kT + t, so loads are coalesced and a warp's ballot is one word of the bit rows).
+// kT threads per row, kV values per thread (value v of thread t is block v * kT + t, so loads
+// are coalesced and a warp's ballot is one word of the bit rows). Bound by HBM for long rows:
+// the scores are read once.
 #include "common.cuh"
 
 namespace tasft {
@@ -24,21 +27,6 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 constexpr uint32_t kNever = 0x007fffffu;  // ordered(-inf): never chosen; below every other score
 
-template <int kT>
-__device__ __forceinline__ int group_count(int n, int32_t* scratch, int parity) {
-  n = __reduce_add_sync(0xffffffffu, n);
-  if constexpr (kT > 32) {
-    // two alternating rows of scratch: one barrier per count
-    int32_t* row = scratch + parity * (kT / 32);
-    if ((threadIdx.x & 31) == 0) row[threadIdx.x >> 5] = n;
-    __syncthreads();
-    n = 0;
-#pragma unroll
-    for (int w = 0; w < kT / 32; ++w) n += row[w];
-  }
-  return n;
-}
-
 // Threads of a block: kT for one row, or four warps with a row each when kT is 32.
 template <int kT, int kV>
 __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(const tasft_select_args a) {
@@ -46,7 +34,6 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
   constexpr int kRowsPerCta = kT == 32 ? 4 : 1;
   __shared__ uint32_t bits_[kRowsPerCta][2 * kWords];  // above the threshold, at it
   __shared__ int32_t place_[kRowsPerCta][kWords + 1];
-  __shared__ int32_t scratch[2 * (kT / 32)];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = kT == 32 ? warp : 0, t = kT == 32 ? lane : threadIdx.x;
   const int64_t row = (int64_t)blockIdx.x * kRowsPerCta + sub;
@@ -74,53 +61,156 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
 
   const float* s = a.scores + b * a.stride[0] + (int64_t)hk * grp * a.stride[1] + (int64_t)i * a.stride[2];
   uint32_t key[kV];
+  {
+    float x[kV];
 #pragma unroll
-  for (int v = 0; v < kV; ++v) {
-    const int j = v * kT + t;
-    key[v] = 0;
-    if (j >= lead && j < tail) {
-      float x = -INFINITY;
-      for (int h = 0; h < grp; ++h) x = fmaxf(x, __ldg(s + h * a.stride[1] + j));  // fmaxf drops NaN
-      if (!a.use_tau || x >= a.tau) key[v] = ordered(x);
+    for (int v = 0; v < kV; ++v) x[v] = -INFINITY;
+#pragma unroll 2
+    for (int h = 0; h < grp; ++h) {
+      const float* sh = s + h * a.stride[1];
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        const int j = v * kT + t;
+        if (j >= lead && j < tail) x[v] = fmaxf(x[v], __ldg(sh + j));  // fmaxf drops NaN
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < kV; ++v) {
+      key[v] = !a.use_tau || x[v] >= a.tau ? ordered(x[v]) : 0u;
       if (key[v] <= kNever) key[v] = 0;
     }
   }
-  // the largest threshold that `want` keys reach (0: they do not, everything above 0 is taken)
-  uint32_t thr = 0;
-  int parity = 0;
-  if (want > 0) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t cand = thr | (1u << bit);
-      int n = 0;
+  // keys from thr on are taken; where `quota` says so, only that many of those at thr itself
+  uint32_t thr = 0xffffffffu;
+  int quota = 0;
+  if constexpr (kT == 32) {
+    if (want > 0) {
+      thr = 0;  // the largest value that `want` keys reach (0: fewer keys than that, all taken)
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = thr | (1u << bit);
+        int n = 0;
 #pragma unroll
-      for (int v = 0; v < kV; ++v) n += key[v] >= cand;
-      n = group_count<kT>(n, scratch, parity);
-      parity ^= 1;
-      if (n >= want) thr = cand;
-      if (n == want) break;  // exactly these: no smaller bit can part them
+        for (int v = 0; v < kV; ++v) n += key[v] >= cand;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n >= want) thr = cand;
+        if (n == want) break;  // exactly these: no smaller bit can part them
+      }
+      if (thr == 0) {
+        thr = 1;
+        quota = INT32_MAX;
+      } else {
+        int n = 0;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) n += key[v] > thr;
+        quota = want - __reduce_add_sync(0xffffffffu, n);
+      }
+    }
+  } else {
+    __shared__ uint32_t red[3][kT / 32];
+    __shared__ int32_t hist[256];
+    __shared__ int32_t part[8];
+    __shared__ int32_t found[3];  // digit, how many of it are wanted, how many there are
+    if (want > 0) {               // the same for the whole CTA
+      uint32_t hi = 0, lo = 0xffffffffu, n = 0;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        hi = max(hi, key[v]);
+        lo = min(lo, key[v] ? key[v] : 0xffffffffu);
+        n += key[v] != 0;
+      }
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) {
+        red[0][warp] = hi;
+        red[1][warp] = lo;
+        red[2][warp] = n;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kT / 32; ++w) {
+        hi = max(hi, red[0][w]);
+        lo = min(lo, red[1][w]);
+        n = (w == 0 ? 0 : n) + red[2][w];
+      }
+      if ((int)n <= want) {
+        thr = 1;
+        quota = INT32_MAX;
+      } else {
+        int left = want;
+        int top = hi == lo ? 0 : 32 - __clz(hi ^ lo);  // bits [0, top) are open
+        thr = top == 32 ? 0u : hi >> top << top;
+        quota = INT32_MAX;
+        while (true) {
+          if (top == 0) {  // all open keys are thr itself
+            quota = left;
+            break;
+          }
+          const int shift = max(0, top - 8);
+          for (int i = t; i < 256; i += kT) hist[i] = 0;
+          __syncthreads();
+#pragma unroll
+          for (int v = 0; v < kV; ++v)
+            if (key[v] && (top == 32 || key[v] >> top == thr >> top))
+              atomicAdd(&hist[(key[v] >> shift) & ((1u << (top - shift)) - 1u)], 1);
+          __syncthreads();
+          // the digit in which the count from the top reaches `left` (256 threads or the first 128,
+          // two digits each)
+          constexpr int kPer = kT >= 256 ? 1 : 256 / kT;
+          int mine_n[kPer], sum = 0, pre = 0;
+          if (t < 256) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) sum += mine_n[i] = hist[255 - (t * kPer + i)];
+            pre = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int x = __shfl_up_sync(0xffffffffu, pre, o);
+              if (lane >= o) pre += x;
+            }
+            if (lane == 31) part[warp] = pre;
+          }
+          __syncthreads();
+          if (t < 256) {
+            for (int w = 0; w < warp; ++w) pre += part[w];
+            int c = pre - sum;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              if (c < left && c + mine_n[i] >= left) {
+                found[0] = 255 - (t * kPer + i);
+                found[1] = left - c;
+                found[2] = mine_n[i];
+              }
+              c += mine_n[i];
+            }
+          }
+          __syncthreads();
+          thr |= (uint32_t)found[0] << shift;
+          left = found[1];
+          if (left == found[2]) break;  // the whole digit is taken
+          top = shift;
+        }
+      }
     }
   }
-  // ---- bits: always kept or above the threshold; at the threshold ----
-  int n_above = 0;
+  // ---- bits: always kept or above the threshold; at the threshold, where not all of those are ----
+  const bool all = quota == INT32_MAX;
 #pragma unroll
   for (int v = 0; v < kV; ++v) {
     const int j = v * kT + t;
     const bool forced = j < lead || (j >= tail && j <= mine);
-    const bool up = want > 0 && key[v] > thr;
-    n_above += up;
+    const bool up = want > 0 && (all ? key[v] >= thr : key[v] > thr);
     const unsigned wa = __ballot_sync(0xffffffffu, forced || up);
-    const unsigned we = __ballot_sync(0xffffffffu, want > 0 && thr > 0 && key[v] == thr);
+    const unsigned we = __ballot_sync(0xffffffffu, want > 0 && !all && key[v] == thr);
     if (lane == 0) {
       above[(v * kT + t) >> 5] = wa;
       at[(v * kT + t) >> 5] = we;
     }
   }
-  n_above = group_count<kT>(n_above, scratch, parity);
   if constexpr (kT > 32) __syncthreads();
   else __syncwarp();
-  // ---- one warp: the first (want - n_above) at the threshold join; places of the words ----
+  // ---- one warp: the first `quota` at the threshold join; places of the words ----
   if (t < 32) {
-    int ties = want - n_above, out = 0;
+    int ties = quota, out = 0;
     for (int w0 = 0; w0 < kWords; w0 += 32) {
       const int w = w0 + lane;
       uint32_t e = w < kWords ? at[w] : 0u, m = w < kWords ? above[w] : 0u;
@@ -132,16 +222,16 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
         if (lane >= o) pre += x;
       }
       const int total = __shfl_sync(0xffffffffu, pre, 31);
-      int quota = min(max(ties - (pre - ne), 0), ne);
-      if (quota == ne) {
+      int join = min(max(ties - (pre - ne), 0), ne);
+      if (join == ne) {
         m |= e;
       } else {
-        for (; quota > 0; --quota) {  // lowest indices first
+        for (; join > 0; --join) {  // lowest indices first
           m |= e & (0u - e);
           e &= e - 1;
         }
       }
-      ties -= total;
+      if (!all) ties -= total;
       const int nk = __popc(m);
       int pk = nk;
 #pragma unroll
