@@ -190,7 +190,8 @@ TASFT_API int tasft_rope_append_paged(const tasft_rope_append_args* args, tasft_
  * the decode calls); a row that no new token falls in keeps nothing. Beside
  * tasft_mask_from_scores: a count instead of a threshold. The reference has no top-k
  * (tasft/modules/attn_gate.py:475). TASFT_DEVERR_INDEX: lengths that do not fit NBq, NBk
- * or each other (the sequence keeps nothing). NBk <= 16384. */
+ * or each other (the sequence keeps nothing). NBk <= 16384,
+ * block a power of two. */
 typedef struct {
   const float* scores;      /* [B, Hq, NBq, NBk] */
   int64_t stride[3];        /* batch, head, row (elements); columns contiguous */

@@ -29,27 +29,38 @@ constexpr uint32_t kNever = 0x007fffffu;  // ordered(-inf): never chosen; below 
 
 // Threads of a block: kT for one row, or four warps with a row each when kT is 32.
 template <int kT, int kV>
-__global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(const tasft_select_args a) {
+__global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(const tasft_select_args a, const int log2_block) {
   constexpr int kWords = kT * kV / 32;
   constexpr int kRowsPerCta = kT == 32 ? 4 : 1;
   __shared__ uint32_t bits_[kRowsPerCta][2 * kWords];  // above the threshold, at it
   __shared__ int32_t place_[kRowsPerCta][kWords + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = kT == 32 ? warp : 0, t = kT == 32 ? lane : threadIdx.x;
-  const int64_t row = (int64_t)blockIdx.x * kRowsPerCta + sub;
-  if (row >= (int64_t)a.B * a.Hk * a.NBq) return;  // whole warps (kT 32) or never
+  // one CTA per row of a (row, kv-head, sequence) grid, or four consecutive rows per CTA
+  int i, hk, b;
+  if constexpr (kT == 32) {
+    const uint32_t r = blockIdx.x * kRowsPerCta + sub, nq = a.NBq, nh = a.Hk;
+    if (r >= (uint32_t)a.B * nh * nq) return;  // whole warps
+    i = r % nq;
+    hk = r / nq % nh;
+    b = r / nq / nh;
+  } else {
+    i = blockIdx.x;
+    hk = blockIdx.y;
+    b = blockIdx.z;
+  }
+  const int64_t row = ((int64_t)b * a.Hk + hk) * a.NBq + i;
   uint32_t* above = bits_[sub];
   uint32_t* at = above + kWords;
   int32_t* place = place_[sub];
-  const int i = (int)(row % a.NBq), hk = (int)(row / a.NBq % a.Hk), b = (int)(row / a.NBq / a.Hk);
   int32_t* idx = a.kept_idx + row * a.width;
   const int grp = a.Hq / a.Hk;
 
   const int n_new = a.cu_seqlens[b + 1] - a.cu_seqlens[b], len = a.kv_len[b];
-  const bool bad = n_new < 0 || (n_new > 0 && (len < n_new || (len - 1) / a.block >= a.NBk ||
-                                               (len - 1) / a.block - (len - n_new) / a.block >= a.NBq));
-  const int mine = n_new > 0 && !bad ? (len - n_new) / a.block + i : 0;
-  if (bad || n_new <= 0 || mine > (len - 1) / a.block) {  // no such row
+  const int own0 = (len - n_new) >> log2_block, own_last = (len - 1) >> log2_block;
+  const bool bad = n_new < 0 || (n_new > 0 && (len < n_new || own_last >= a.NBk || own_last - own0 >= a.NBq));
+  const int mine = own0 + i;
+  if (bad || n_new <= 0 || mine > own_last) {  // no such row
     if (bad && t == 0) set_err(a.err, TASFT_DEVERR_INDEX);
     for (int j = t; j < a.width; j += kT) idx[j] = -1;
     if (t == 0) a.kept_cnt[row] = 0;
@@ -65,19 +76,25 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
     float x[kV];
 #pragma unroll
     for (int v = 0; v < kV; ++v) x[v] = -INFINITY;
-#pragma unroll 2
-    for (int h = 0; h < grp; ++h) {
-      const float* sh = s + h * a.stride[1];
+    if (want > 0) {
+      for (int h = 0; h < grp; h += 4) {  // four heads' loads go out together
+        float y[4][kV];
 #pragma unroll
-      for (int v = 0; v < kV; ++v) {
-        const int j = v * kT + t;
-        if (j >= lead && j < tail) x[v] = fmaxf(x[v], __ldg(sh + j));  // fmaxf drops NaN
+        for (int g = 0; g < 4; ++g) {
+          const float* sh = s + min(h + g, grp - 1) * a.stride[1] + t;
+#pragma unroll
+          for (int v = 0; v < kV; ++v) y[g][v] = v * kT + t < tail ? __ldg(sh + v * kT) : -INFINITY;
+        }
+#pragma unroll
+        for (int v = 0; v < kV; ++v)  // fmaxf drops NaN
+          x[v] = fmaxf(x[v], fmaxf(fmaxf(y[0][v], y[1][v]), fmaxf(y[2][v], y[3][v])));
       }
     }
 #pragma unroll
     for (int v = 0; v < kV; ++v) {
+      const int j = v * kT + t;
       key[v] = !a.use_tau || x[v] >= a.tau ? ordered(x[v]) : 0u;
-      if (key[v] <= kNever) key[v] = 0;
+      if (key[v] <= kNever || j < lead || j >= tail) key[v] = 0;
     }
   }
   // keys from thr on are taken; where `quota` says so, only that many of those at thr itself
@@ -264,9 +281,11 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
 template <int kT, int kV>
 int run(const tasft_select_args& a, cudaStream_t st) {
   const int64_t rows = (int64_t)a.B * a.Hk * a.NBq;
-  const int64_t ctas = kT == 32 ? (rows + 3) / 4 : rows;
-  if (ctas > INT32_MAX) return TASFT_ERR_TOO_LARGE;
-  select_blocks_kernel<kT, kV><<<(unsigned)ctas, kT == 32 ? 128 : kT, 0, st>>>(a);
+  if (rows > INT32_MAX / 2 || a.B > 65535 || a.Hk > 65535) return TASFT_ERR_TOO_LARGE;
+  const dim3 grid = kT == 32 ? dim3((unsigned)((rows + 3) / 4)) : dim3((unsigned)a.NBq, (unsigned)a.Hk, (unsigned)a.B);
+  int log2_block = 0;
+  while ((1 << log2_block) < a.block) ++log2_block;
+  select_blocks_kernel<kT, kV><<<grid, kT == 32 ? 128 : kT, 0, st>>>(a, log2_block);
   count_launch();
   return launch_status();
 }
@@ -283,6 +302,7 @@ extern "C" int tasft_select_blocks(const tasft_select_args* ap, tasft_stream_t s
   if (a.B <= 0 || a.Hq <= 0 || a.Hk <= 0 || a.Hq % a.Hk || a.NBq <= 0 || a.NBk <= 0 || a.block <= 0)
     return TASFT_ERR_INVALID_ARG;
   if (a.top_k <= 0 || a.first < 0 || a.local < 1 || a.width <= 0) return TASFT_ERR_INVALID_ARG;
+  if (a.block & (a.block - 1)) return TASFT_ERR_UNSUPPORTED;
   // a row never keeps more than this, so a list never runs over its row
   const int64_t most = a.first + (int64_t)a.local > a.top_k ? a.first + (int64_t)a.local : a.top_k;
   if (a.width < (most < a.NBk ? most : a.NBk)) return TASFT_ERR_INVALID_ARG;

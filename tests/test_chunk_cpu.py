@@ -86,7 +86,7 @@ def select_args(**kw):
 @pytest.mark.parametrize("change,status", [
     (dict(scores=None), -1), (dict(kept_cnt=None), -1), (dict(B=0), -1), (dict(Hq=9), -1), (dict(NBk=0), -1),
     (dict(top_k=0), -1), (dict(first=-1), -1), (dict(local=0), -1), (dict(width=7), -1), (dict(first=9, width=9), -1),
-    (dict(NBk=16385, width=8), -5),
+    (dict(NBk=16385, width=8), -5), (dict(block=48), -2), (dict(B=70000), -5),
 ])
 def test_select_refusals(change, status):
     assert L.lib().tasft_select_blocks(C.byref(select_args(**change)), None) == status
