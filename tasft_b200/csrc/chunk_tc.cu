@@ -24,8 +24,10 @@
 //         P read from TMEM where it overwrote S)
 //   2     lists: the next segment (at most kSeg entries) of block indices with their pages,
 //         double-buffered, ahead of the producer
-//   3     idle: warps 0-3 hand registers to the second warpgroup (128 -> 96 and 160 a thread)
+//   3     idle
 //   4-7   softmax, one thread per row; epilogue
+// Warps 0-3 hand registers to the second warpgroup (128 -> 96 and 160 a thread), each role at its
+// start: the compiler gives the code behind a common point the smaller count and spills.
 // Rows of V that no key stands for (past kv_len, or of a page that is not there) are zeroed in
 // shared memory before P.V, so what the cache holds there never meets a 0 of P.
 // Every mbarrier phase is indexed by a global counter and every wait is arranged so the waiter
@@ -74,6 +76,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// One arrival for the warp: what its lanes did before is released by lane 0. (32 lanes that
+// arrive one by one on the same barrier take some 500 cycles.)
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  tc::tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 
 // One list segment and the tile it belongs to.
@@ -137,12 +147,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* k_full = bars + 2;       // [2] per block
   uint64_t* k_empty = bars + 4;      // [2] per block: S(g) has run
   uint64_t* s_full = bars + 6;       // [2] per block
-  uint64_t* p_ready = bars + 8;      // [2] per block (128 arrivals)
+  uint64_t* p_ready = bars + 8;      // [2] per block (one arrival per softmax warp)
   uint64_t* pv_done = bars + 10;     // [2] per block: P.V(g) has run
   uint64_t* o_final = bars + 12;     // per tile: O complete
-  uint64_t* o_free = bars + 13;      // per tile: epilogue has read O (128 arrivals)
+  uint64_t* o_free = bars + 13;      // per tile: epilogue has read O (one arrival per warp)
   uint64_t* list_full = bars + 14;   // [2] per segment
-  uint64_t* list_empty = bars + 16;  // [2] per segment (128 arrivals)
+  uint64_t* list_empty = bars + 16;  // [2] per segment (one arrival per softmax warp)
   uint64_t* v_full = bars + 18;      // [2] per block
   uint64_t* v_empty = bars + 20;     // [2] per block: P.V(g) has run
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
@@ -159,13 +169,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 128);
+      mbar_init(&p_ready[i], 4);
       mbar_init(&pv_done[i], 1);
       mbar_init(&list_full[i], 1);
-      mbar_init(&list_empty[i], 128);
+      mbar_init(&list_empty[i], 4);
     }
     mbar_init(o_final, 1);
-    mbar_init(o_free, 128);
+    mbar_init(o_free, 4);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -181,11 +191,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tS0 = tmem;       // S buffers: columns [0,64) and [64,128)
   const uint32_t tO = tmem + 128;  // O: columns [128, 128 + D)
 
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-
   if (warp == 2) {
     // ================= lists =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     int32_t* item0 = reinterpret_cast<int32_t*>(smem + L::kItemOff);
     int32_t* slot0 = reinterpret_cast<int32_t*>(smem + L::kSlotOff);
     uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + L::kBitmapOff);
@@ -461,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 0) {
     // ================= producer =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (lane == 0) {
       tc::prefetch_tmap(&tmq);
       tc::prefetch_tmap(&tmk);
@@ -527,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 1) {
     // ================= MMA issuer =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (lane == 0) {
       constexpr uint32_t fmt = kF16 ? 0u : 1u;
       constexpr uint32_t idesc_s = tc::make_idesc(128, 64, fmt, false);
@@ -599,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp >= 4) {
     // ================= softmax + epilogue (warps 4..7) =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     const int quarter = warp & 3;       // TMEM lanes [32*quarter, 32*quarter + 32)
     const int r = quarter * 32 + lane;  // tile row
     const int slot = sh.mode == 2 ? r >> 6 : 0;
@@ -721,8 +732,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           fence_proxy_async_smem();
         }
-        tc::tc_fence_before();
-        mbar_arrive(&p_ready[gi & 1]);
+        warp_arrive(&p_ready[gi & 1], lane);
         started = true;
       }
       if (!ok) break;
@@ -773,12 +783,13 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        tc::tc_fence_before();
-        mbar_arrive(o_free);
+        warp_arrive(o_free, lane);
       }
-      mbar_arrive(&list_empty[lb]);
+      warp_arrive(&list_empty[lb], lane);
     }
     if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 12));
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   }
   // ---------------- teardown ----------------
   __syncwarp();
