@@ -9,6 +9,7 @@ namespace tasft {
 constexpr int kChunkBlk = 64;          // block size (tokens) of the kept lists
 constexpr int kChunkMaxSplits = 128;   // most items one tile is cut into
 constexpr int kChunkMinPiece = 4;      // fewest blocks an item is cut down to
+constexpr int kChunkMergeCost = 10;    // what a cut costs (partials, merge), in blocks
 constexpr int kChunkBuckets = 256;     // entries of the per-CTA prefix over sequences
 
 // Launch-wide choices the host makes from types and sizes.
@@ -16,7 +17,7 @@ struct ChunkShape {
   int mode;       // how the 128 rows of a tile are filled, see chunk_tc.cu
   int hpt, tpt;   // query heads and tokens of a tile (mode 2: unused)
   int units;      // tiles beside one another at the same tokens (kv-heads, or pairs of query heads)
-  int bound;      // most blocks a row can visit: list width, or capacity of the block table
+  int tpt_log2;   // modes 1 and 2
   int capacity;   // tokens the block table can hold (max_pages * page_size)
   int slots;      // split items the workspace has room for
   int rows;       // rows of a split item's partials
@@ -32,7 +33,7 @@ struct ChunkWs {
 
 struct ChunkSeq {
   int start, n, ctx, len;  // first row of its new tokens, how many, tokens before them, all tokens
-  int tiles, cost;         // tiles per unit; most blocks one tile visits
+  int tiles;               // per unit
   bool bad;
 };
 
@@ -48,31 +49,35 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const tasft_chunk_args& a, const C
     s.n = 0;
   }
   s.ctx = s.n > 0 ? s.len - s.n : 0;
-  if (s.n == 0) {
-    s.tiles = s.cost = 0;
-  } else {
+  s.tiles = 0;
+  if (s.n > 0) {
     if (sh.mode == 0) {
-      s.tiles = (s.n + sh.tpt - 1) / sh.tpt;
+      s.tiles = (uint32_t)(s.n + sh.tpt - 1) / (uint32_t)sh.tpt;
     } else {
       // tiles stand at multiples of their token count, so none spans two rows of the lists
       // (mode 2 with one head per kv-head: two rows on purpose)
-      s.tiles = (s.len - 1) / sh.tpt - s.ctx / sh.tpt + 1;
+      s.tiles = ((s.len - 1) >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2) + 1;
     }
-    s.cost = min((s.len + kChunkBlk - 1) / kChunkBlk, sh.bound);
   }
   return s;
 }
 
-// Items a tile of this sequence is cut into, for pieces of about `target` blocks.
-__device__ __forceinline__ int chunk_splits(const ChunkSeq& s, int target) {
-  return s.n == 0 ? 1 : max(1, min(kChunkMaxSplits, (s.cost + target - 1) / target));
+// Blocks a tile of the sequence visits, for balance alone: those up to its last token, or the
+// length of that token's list (first head; mode 2 walks two lists).
+__device__ __forceinline__ int chunk_cost(const tasft_chunk_args& a, const ChunkShape& sh, const ChunkSeq& s, int b) {
+  if (s.n == 0) return 0;
+  const int last = (s.len - 1) / kChunkBlk;
+  if (sh.mode == 0) return last + 1;
+  const int cnt = a.kept_cnt[(int64_t)b * a.Hm * a.nb_q + (last - s.ctx / kChunkBlk)];
+  return min(max(cnt, 0) * (sh.mode == 2 ? 2 : 1), last + 1);
 }
 
-__device__ __forceinline__ int warp_sum_int(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Items a tile is cut into, for pieces of about `target` blocks.
+__device__ __forceinline__ int chunk_splits(int cost, int target) {
+  if (cost <= target + kChunkMergeCost) return 1;
+  return min(kChunkMaxSplits, (int)((uint32_t)(cost + target - 1) / (uint32_t)target));
 }
+
 __device__ __forceinline__ int warp_scan_int(int v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {

@@ -26,7 +26,7 @@
 //         double-buffered, ahead of the producer
 //   3     idle
 //   4-7   softmax, one thread per row; epilogue
-// Warps 0-3 hand registers to the second warpgroup (128 -> 96 and 160 a thread), each role at its
+// Warps 0-3 hand registers to the second warpgroup (128 -> 88 and 168 a thread), each role at its
 // start: the compiler gives the code behind a common point the smaller count and spills.
 // Rows of V that no key stands for (past kv_len, or of a page that is not there) are zeroed in
 // shared memory before P.V, so what the cache holds there never meets a 0 of P.
@@ -114,7 +114,8 @@ struct Smem {
   static constexpr int kPageOff = kListOff + 2 * kSeg * 4;       // [2][kSeg][4] pages
   static constexpr int kItemOff = kPageOff + 2 * kSeg * 16;      // [kChunkBuckets + 1] first item
   static constexpr int kSlotOff = kItemOff + (kChunkBuckets + 1) * 4;  // the same, first split slot
-  static constexpr int kBitmapOff = kSlotOff + (kChunkBuckets + 1) * 4;  // [2][kSeg / 32]
+  static constexpr int kSeqOff = (kSlotOff + (kChunkBuckets + 1) * 4 + 15) / 16 * 16;  // [kChunkBuckets] int4
+  static constexpr int kBitmapOff = kSeqOff + kChunkBuckets * 16;  // [2][kSeg / 32]
   static constexpr int kWorkOff = (kBitmapOff + 2 * (kSeg / 32) * 4 + 7) / 8 * 8;
   static constexpr int kBarOff = (kWorkOff + 2 * (int)sizeof(Work) + 7) / 8 * 8;
   static constexpr int kNumBars = 22;
@@ -182,40 +183,37 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc::tmem_alloc(&misc[0], kTmemCols);
     tc::tmem_relinquish();
   }
-  tc::tc_fence_before();
-  __syncthreads();
-  tc::tc_fence_after();
-  // the merge kernel behind this one waits for this grid before it reads anything
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const uint32_t tmem = misc[0];
-  const uint32_t tS0 = tmem;       // S buffers: columns [0,64) and [64,128)
-  const uint32_t tO = tmem + 128;  // O: columns [128, 128 + D)
-
+  int32_t* item0 = reinterpret_cast<int32_t*>(smem + L::kItemOff);
+  int32_t* slot0 = reinterpret_cast<int32_t*>(smem + L::kSlotOff);
+  int4* seqs = reinterpret_cast<int4*>(smem + L::kSeqOff);  // start, n, len, splits (stride 1)
+  int items = 0, target = 0;
   if (warp == 2) {
-    // ================= lists =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    int32_t* item0 = reinterpret_cast<int32_t*>(smem + L::kItemOff);
-    int32_t* slot0 = reinterpret_cast<int32_t*>(smem + L::kSlotOff);
-    uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + L::kBitmapOff);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- cut the batch into items: pieces of about the mean load of a CTA ----
     float load = 0.f;
+    ChunkSeq s = {};
+    int cost = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       const int b = b0 + lane;
       if (b < a.B) {
-        const ChunkSeq s = chunk_seq(a, sh, b);
-        load += (float)s.tiles * (float)s.cost;
+        s = chunk_seq(a, sh, b);
+        cost = chunk_cost(a, sh, s, b);
+        load += (float)s.tiles * (float)cost;
         if (s.bad && blockIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
       }
     }
     load = warp_sum(load) * (float)sh.units;
-    const int target = max(kChunkMinPiece, (int)ceilf(load / (float)gridDim.x));
-    int items = 0, slots = 0;
+    target = max(kChunkMinPiece, (int)ceilf(load / (float)gridDim.x));
+    int slots = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       const int b = b0 + lane;
       int it = 0, sl = 0, ns = 1;
       if (b < a.B) {
-        const ChunkSeq s = chunk_seq(a, sh, b);
-        ns = chunk_splits(s, target);
+        if (a.B > 32) {  // else the lane's own sequence is still at hand
+          s = chunk_seq(a, sh, b);
+          cost = chunk_cost(a, sh, s, b);
+        }
+        ns = chunk_splits(cost, target);
         it = s.tiles * sh.units;
         sl = ns > 1 ? it * ns : 0;
       }
@@ -225,9 +223,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (slots + fs > sh.slots) ns = 1;
       const int fi = warp_scan_int(it * ns, lane);
       if (b < a.B) {
-        if (b % sh.stride == 0) {
-          item0[b / sh.stride] = items + fi - it * ns;
-          slot0[b / sh.stride] = slots + fs - sl;
+        if (sh.stride == 1 || b % sh.stride == 0) {
+          const int at = sh.stride == 1 ? b : b / sh.stride;
+          item0[at] = items + fi - it * ns;
+          slot0[at] = slots + fs - sl;
+          if (sh.stride == 1) seqs[at] = make_int4(s.start, s.n, s.len, ns);
         }
         if (blockIdx.x == 0) ws.plan[b] = make_int2(ns, slots + fs - sl);
       }
@@ -235,6 +235,22 @@ __global__ void __launch_bounds__(kThreads, 2)
       slots += __shfl_sync(0xffffffffu, fs, 31);
     }
     __syncwarp();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  // nothing above touched memory that the kernel before this one may still use (warp 2 waited)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the merge kernel behind this one waits for this grid before it reads anything
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = misc[0];
+  const uint32_t tS0 = tmem;       // S buffers: columns [0,64) and [64,128)
+  const uint32_t tO = tmem + 128;  // O: columns [128, 128 + D)
+
+  if (warp == 2) {
+    // ================= lists =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + L::kBitmapOff);
     const int buckets = (a.B + sh.stride - 1) / sh.stride;
     const PagedGeo geo = {max(1, kChunkBlk / a.page_size), min(kChunkBlk, a.page_size)};
 
@@ -260,27 +276,38 @@ __global__ void __launch_bounds__(kThreads, 2)
         int first_item = item0[bl], first_slot = slot0[bl];
         ChunkSeq s;
         int ns;
-        while (true) {
-          s = chunk_seq(a, sh, b);
-          ns = chunk_splits(s, target);
-          const int it = s.tiles * sh.units, ask = ns > 1 ? it * ns : 0;
-          if (first_slot + ask > sh.slots) ns = 1;
-          if (item < first_item + it * ns || b + 1 >= a.B) break;
-          first_item += it * ns;
-          first_slot += ask;
-          ++b;
+        if (sh.stride == 1) {
+          const int4 q4 = seqs[b];
+          s.start = q4.x;
+          s.n = q4.y;
+          s.len = q4.z;
+          s.ctx = s.len - s.n;
+          ns = q4.w;
+          s.tiles = sh.mode == 0 ? (int)((uint32_t)(s.n + sh.tpt - 1) / (uint32_t)sh.tpt)
+                                 : ((s.len - 1) >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2) + 1;
+        } else {
+          while (true) {
+            s = chunk_seq(a, sh, b);
+            ns = chunk_splits(chunk_cost(a, sh, s, b), target);
+            const int it = s.tiles * sh.units, ask = ns > 1 ? it * ns : 0;
+            if (first_slot + ask > sh.slots) ns = 1;
+            if (item < first_item + it * ns || b + 1 >= a.B) break;
+            first_item += it * ns;
+            first_slot += ask;
+            ++b;
+          }
         }
-        int rest = item - first_item;
-        const int unit = rest % sh.units;
-        rest /= sh.units;
-        const int split = rest % ns;
-        const int tile = s.tiles - 1 - rest / ns;
+        const uint32_t rest = (uint32_t)(item - first_item) / (uint32_t)sh.units;
+        const int unit = item - first_item - (int)rest * sh.units;
+        const uint32_t back = ns == 1 ? rest : rest / (uint32_t)ns;
+        const int split = (int)(rest - back * ns);
+        const int tile = s.tiles - 1 - (int)back;
         w.len = s.len;
         w.ctx = s.ctx;
         w.part = ns > 1 ? first_slot + (tile * sh.units + unit) * ns + split : -1;
         int diag;  // last block the tile may visit
         if (sh.mode == 2) {
-          const int base = (s.ctx / sh.tpt + tile) * sh.tpt;
+          const int base = ((s.ctx >> sh.tpt_log2) + tile) << sh.tpt_log2;
           if (grp >= 2) {
             const int pairs = (grp + 1) / 2, p = unit % pairs;
             w.hk = unit / pairs;
@@ -311,9 +338,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             cnt[x] = min(max(a.kept_cnt[lrow], 0), a.nb_w);
             idx[x] = a.kept_idx + lrow * a.nb_w;
           }
-          // slices by block index
-          lo = (int)((int64_t)split * (diag + 1) / ns);
-          hi = (int)((int64_t)(split + 1) * (diag + 1) / ns);
+          // (its slices are ranges of block indices)
+          lo = 0;
+          hi = diag + 1;
         } else {
           w.hk = unit;
           w.head[0] = w.head[1] = unit * grp;
@@ -322,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             p0 = s.ctx + tile * sh.tpt;
             p1 = min(p0 + sh.tpt, s.len);
           } else {
-            p0 = (s.ctx / sh.tpt + tile) * sh.tpt;
+            p0 = ((s.ctx >> sh.tpt_log2) + tile) << sh.tpt_log2;
             p1 = min(p0 + sh.tpt, s.len);
             p0 = max(p0, s.ctx);
           }
@@ -338,8 +365,12 @@ __global__ void __launch_bounds__(kThreads, 2)
             cnt[0] = min(max(a.kept_cnt[lrow], 0), a.nb_w);
             idx[0] = a.kept_idx + lrow * a.nb_w;
           }
-          lo = (int)((int64_t)split * cnt[0] / ns);
-          hi = (int)((int64_t)(split + 1) * cnt[0] / ns);
+          lo = 0;
+          hi = cnt[0];
+        }
+        if (ns > 1) {  // at most 2^20 blocks in 2^7 slices
+          lo = (int)((uint32_t)(split * hi) / (uint32_t)ns);
+          hi = (int)((uint32_t)((split + 1) * hi) / (uint32_t)ns);
         }
       }
       // ---- the item's segments ----
@@ -469,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 0) {
     // ================= producer =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (lane == 0) {
       tc::prefetch_tmap(&tmq);
       tc::prefetch_tmap(&tmk);
@@ -536,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 1) {
     // ================= MMA issuer =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (lane == 0) {
       constexpr uint32_t fmt = kF16 ? 0u : 1u;
       constexpr uint32_t idesc_s = tc::make_idesc(128, 64, fmt, false);
@@ -609,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp >= 4) {
     // ================= softmax + epilogue (warps 4..7) =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int quarter = warp & 3;       // TMEM lanes [32*quarter, 32*quarter + 32)
     const int r = quarter * 32 + lane;  // tile row
     const int slot = sh.mode == 2 ? r >> 6 : 0;
@@ -632,6 +663,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int32_t* list = lists + lb * kSeg;
       const int qpos = w->pos[slot] + tok;
       const bool live = sh.mode == 2 ? w->valid[slot] && qpos >= w->ctx && qpos < len : tok < w->valid[0];
+      // a warp whose rows hold no token only keeps the barriers going: what P and O hold in its
+      // rows meets nothing else
+      const bool any_live = __any_sync(0xffffffffu, live);
       if (w->first) {
         ++tile;
         started = false;
@@ -645,81 +679,83 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int entry = list[j];
         const int kbase = (entry & kKbMask) * kChunkBlk;
         const int have = (entry >> kKbBits) & 15;
-        uint32_t sraw[64];
-        tc::tmem_ld64_sync(tS0 + (gi & 1) * 64 + lane_off, sraw);
-        // keys this row may see: up to its own position
-        int lim = qpos - kbase + 1;
-        if (!live || !((entry >> (kKbBits + 4 + slot)) & 1)) lim = 0;
-        lim = max(0, min(lim, kChunkBlk));
-        float sv[64];
+        if (any_live) {
+          uint32_t sraw[64];
+          tc::tmem_ld64_sync(tS0 + (gi & 1) * 64 + lane_off, sraw);
+          // keys this row may see: up to its own position
+          int lim = qpos - kbase + 1;
+          if (!live || !((entry >> (kKbBits + 4 + slot)) & 1)) lim = 0;
+          lim = max(0, min(lim, kChunkBlk));
+          float sv[64];
 #pragma unroll
-        for (int c = 0; c < 64; ++c) sv[c] = __uint_as_float(sraw[c]);
-        if (__any_sync(0xffffffffu, lim < kChunkBlk)) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (c >= lim) sv[c] = -INFINITY;
-        }
-        if (have != all_pages) {  // keys of a page that is not there
-          uint64_t seen = 0;
-          for (int x = 0; x * sub_rows < kChunkBlk; ++x)
-            if ((have >> x) & 1) seen |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (!((seen >> c) & 1)) sv[c] = -INFINITY;
-        }
-        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 64; c += 8) {
-#pragma unroll
-          for (int qd = 0; qd < 4; ++qd) mq[qd] = max3(mq[qd], sv[c + 2 * qd], sv[c + 2 * qd + 1]);
-        }
-        const float mb = max3(mq[0], mq[1], fmaxf(mq[2], mq[3]));
-        const float m_new = fmaxf(m, mb * sl2);
-        const bool need = (m != -INFINITY) && (m_new > m + kRescaleThreshold);
-        if (m == -INFINITY) m = m_new;  // O row is still exactly zero: no rescale
-        if (__any_sync(0xffffffffu, need)) {
-          // O must hold every earlier P.V of this tile before it is rescaled
-          if (!warp_wait(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1)) { ok = false; break; }
-          tc::tc_fence_after();
-          const float alpha = need ? ex2(m - m_new) : 1.0f;
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            tc::tmem_ld32_sync(tO + c0 + lane_off, o);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-            tc::tmem_st32(tO + c0 + lane_off, o);
-          }
-          tc::tmem_wait_st();
-          if (need) {
-            l *= alpha;
-            m = m_new;
-          }
-        }
-        uint32_t pk[32];
-        float rs = 0.f;
-        if (m == -INFINITY) {  // nothing to see yet, or only scores that are NaN
-#pragma unroll
-          for (int c = 0; c < 32; ++c) pk[c] = 0u;
-          if (lim > 0) {
+          for (int c = 0; c < 64; ++c) sv[c] = __uint_as_float(sraw[c]);
+          if (__any_sync(0xffffffffu, lim < kChunkBlk)) {
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if (sv[c] != sv[c]) rs = sv[c];
+              if (c >= lim) sv[c] = -INFINITY;
           }
-        } else {
-          const uint64_t sc2 = f2(sl2, sl2), nm2 = f2(-m, -m);
-          uint64_t rs2 = 0;
+          if (have != all_pages) {  // keys of a page that is not there
+            uint64_t seen = 0;
+            for (int x = 0; x * sub_rows < kChunkBlk; ++x)
+              if ((have >> x) & 1) seen |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const uint64_t x2 = fma2(f2(sv[2 * c], sv[2 * c + 1]), sc2, nm2);  // s * scale - m
-            const uint64_t p2 = f2(ex2(lo_f(x2)), ex2(hi_f(x2)));
-            rs2 = add2(rs2, p2);
-            pk[c] = kF16 ? tc::pack_f16x2(lo_f(p2), hi_f(p2)) : tc::pack_bf16x2(lo_f(p2), hi_f(p2));
+            for (int c = 0; c < 64; ++c)
+              if (!((seen >> c) & 1)) sv[c] = -INFINITY;
           }
-          rs = lo_f(rs2) + hi_f(rs2);
+          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+            for (int qd = 0; qd < 4; ++qd) mq[qd] = max3(mq[qd], sv[c + 2 * qd], sv[c + 2 * qd + 1]);
+          }
+          const float mb = max3(mq[0], mq[1], fmaxf(mq[2], mq[3]));
+          const float m_new = fmaxf(m, mb * sl2);
+          const bool need = (m != -INFINITY) && (m_new > m + kRescaleThreshold);
+          if (m == -INFINITY) m = m_new;  // O row is still exactly zero: no rescale
+          if (__any_sync(0xffffffffu, need)) {
+            // O must hold every earlier P.V of this tile before it is rescaled
+            if (!warp_wait(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1)) { ok = false; break; }
+            tc::tc_fence_after();
+            const float alpha = need ? ex2(m - m_new) : 1.0f;
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t o[32];
+              tc::tmem_ld32_sync(tO + c0 + lane_off, o);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+              tc::tmem_st32(tO + c0 + lane_off, o);
+            }
+            tc::tmem_wait_st();
+            if (need) {
+              l *= alpha;
+              m = m_new;
+            }
+          }
+          uint32_t pk[32];
+          float rs = 0.f;
+          if (m == -INFINITY) {  // nothing to see yet, or only scores that are NaN
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pk[c] = 0u;
+            if (lim > 0) {
+#pragma unroll
+              for (int c = 0; c < 64; ++c)
+                if (sv[c] != sv[c]) rs = sv[c];
+            }
+          } else {
+            const uint64_t sc2 = f2(sl2, sl2), nm2 = f2(-m, -m);
+            uint64_t rs2 = 0;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const uint64_t x2 = fma2(f2(sv[2 * c], sv[2 * c + 1]), sc2, nm2);  // s * scale - m
+              const uint64_t p2 = f2(ex2(lo_f(x2)), ex2(hi_f(x2)));
+              rs2 = add2(rs2, p2);
+              pk[c] = kF16 ? tc::pack_f16x2(lo_f(p2), hi_f(p2)) : tc::pack_bf16x2(lo_f(p2), hi_f(p2));
+            }
+            rs = lo_f(rs2) + hi_f(rs2);
+          }
+          l += rs;
+          tc::tmem_st32(tS0 + (gi & 1) * 64 + lane_off, pk);
+          tc::tmem_wait_st();
         }
-        l += rs;
-        tc::tmem_st32(tS0 + (gi & 1) * 64 + lane_off, pk);
-        tc::tmem_wait_st();
         if (have != all_pages || kbase + kChunkBlk > len) {
           // rows of V that stand for no key are zeroed (V(gi + 2) cannot land before this
           // block's P.V, which waits for these threads: the wait below is at most a phase behind)
@@ -740,8 +776,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (last) {
         if (!warp_wait(o_final, tile & 1)) { ok = false; break; }
         tc::tc_fence_after();
-        const bool direct = w->part < 0;
-        if (direct) {
+        if (!any_live) {
+        } else if (w->part < 0) {
           T* orow = reinterpret_cast<T*>(a.out) + (int64_t)(w->row[slot] + tok) * a.o_stride[0] +
                     (int64_t)(w->head[slot] + hd) * a.o_stride[1];
           const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that kept nothing gives 0
@@ -789,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 12));
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
   // ---------------- teardown ----------------
   __syncwarp();
@@ -808,6 +844,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const tasft_chunk_args
   using T = typename std::conditional<kF16, __half, __nv_bfloat16>::type;
   constexpr int V = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int grp = a.Hq / a.Hk;
   const int64_t rows = (int64_t)a.T * a.Hq;
@@ -828,7 +865,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const tasft_chunk_args
     const int pos = s.ctx + t - s.start, hk = head / grp, hg = head % grp;
     int tile, unit, row;
     if (sh.mode == 2) {
-      tile = pos / sh.tpt - s.ctx / sh.tpt;
+      tile = (pos >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2);
       unit = grp >= 2 ? hk * ((grp + 1) / 2) + hg / 2 : hk;
       row = grp >= 2 ? (hg & 1) * 64 + (pos & 63) : pos & 127;
     } else {
@@ -837,31 +874,49 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const tasft_chunk_args
         tile = (t - s.start) / sh.tpt;
         row = (t - s.start - tile * sh.tpt) * sh.hpt + hg;
       } else {
-        tile = pos / sh.tpt - s.ctx / sh.tpt;
-        row = (pos - max(s.ctx, (pos / sh.tpt) * sh.tpt)) * sh.hpt + hg;
+        tile = (pos >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2);
+        row = (pos - max(s.ctx, pos >> sh.tpt_log2 << sh.tpt_log2)) * sh.hpt + hg;
       }
     }
     const int64_t part = plan.y + (int64_t)(tile * sh.units + unit) * ns;
+    // lane x holds slice x's weight; the slices' O, eight loads in flight, are added in order
     float M = -INFINITY;
     for (int x = lane; x < ns; x += 32) M = fmaxf(M, ws.ml[(part + x) * sh.rows + row].x);
     M = warp_max(M);
     float acc[V], sum = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) acc[c] = 0.f;
-#pragma unroll 4
-    for (int x = 0; x < ns; ++x) {
-      const int64_t pr = (part + x) * sh.rows + row;
-      const float2 ml = ws.ml[pr];
-      if (ml.y == 0.f) continue;  // a slice with nothing to see wrote no O
-      const float wgt = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
-      sum += wgt * ml.y;
-      const float* o = ws.o + pr * D + lane * V;
-      if constexpr (V == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(o);
-        acc[0] += wgt * v.x; acc[1] += wgt * v.y; acc[2] += wgt * v.z; acc[3] += wgt * v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(o);
-        acc[0] += wgt * v.x; acc[1] += wgt * v.y;
+    for (int x0 = 0; x0 < ns; x0 += 32) {
+      float wgt = 0.f, lw = 0.f;
+      if (x0 + lane < ns) {
+        const float2 ml = ws.ml[(part + x0 + lane) * sh.rows + row];
+        if (ml.y != 0.f) {  // a slice with nothing to see wrote no O
+          wgt = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
+          lw = wgt * ml.y;
+        }
+      }
+      const unsigned have = __ballot_sync(0xffffffffu, lw != 0.f || wgt != 0.f);
+      const int nx = min(32, ns - x0);
+      for (int x1 = 0; x1 < nx; x1 += 8) {
+        float v[8][V];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) v[x][c] = 0.f;
+          if (x1 + x < nx && ((have >> (x1 + x)) & 1)) {
+            const float* o = ws.o + ((part + x0 + x1 + x) * sh.rows + row) * D + lane * V;
+            if constexpr (V == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(o);
+            else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(o);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          if (x1 + x >= nx) break;
+          const float w = __shfl_sync(0xffffffffu, wgt, x1 + x);
+          sum += __shfl_sync(0xffffffffu, lw, x1 + x);
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[c] += w * v[x][c];
+        }
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -898,6 +953,8 @@ bool chunk_shape(ChunkShape& sh, int Hq, int Hk, int Hm, int max_q) {
     }
     sh.rows = grp * (max_q < sh.tpt ? max_q : sh.tpt);
   }
+  sh.tpt_log2 = 0;
+  while ((1 << sh.tpt_log2) < sh.tpt) ++sh.tpt_log2;
   return true;
 }
 
@@ -924,19 +981,24 @@ int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
   ws.o = reinterpret_cast<float*>(p + plan_bytes(a.B) + ((int64_t)sh.slots * sh.rows * 8 + 255) / 256 * 256);
   const int grid = 2 * sms;  // persistent: two CTAs per SM
   if (debug_enabled()) debug_log("chunk_tc D=%d mode=%d grid=%d slots=%d smem=%d", D, sh.mode, grid, sh.slots, smem);
-  kern<<<grid, kThreads, smem, st>>>(mq, mk, mv, a, sh, ws);
-  count_launch();
-  int rc = launch_status();
-  if (rc != TASFT_OK || sh.slots == 0) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)sms * 2);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
+  // both launches may begin while the kernel before them ends; they wait for it on the device
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  int rc = cuda_status(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, a, sh, ws));
+  count_launch();
+  if (rc != TASFT_OK || sh.slots == 0) return rc;
+  const int64_t rows = (int64_t)a.T * a.Hq;
+  cfg.gridDim = dim3((unsigned)(rows / 8 + 1 < 4LL * sms ? rows / 8 + 1 : 4LL * sms));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
   rc = cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<D, kF16>, a, sh, ws));
   count_launch();
   return rc;
@@ -989,13 +1051,14 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   ChunkShape sh;
   if (!chunk_shape(sh, a.Hq, a.Hk, a.kept_idx ? a.Hm : 0, a.max_q)) return TASFT_ERR_UNSUPPORTED;
   sh.capacity = a.max_pages * a.page_size;
-  const int blocks = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
-  sh.bound = a.kept_idx && a.nb_w * (sh.mode == 2 ? 2 : 1) < blocks ? a.nb_w * (sh.mode == 2 ? 2 : 1) : blocks;
+  // most blocks a tile visits
+  int bound = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
+  if (a.kept_idx && (int64_t)a.nb_w * 2 < bound) bound = a.nb_w * (sh.mode == 2 ? 2 : 1);
   sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
   if (!a.workspace || a.workspace_bytes < plan_bytes(a.B)) return TASFT_ERR_WORKSPACE;
   const int64_t slots = (a.workspace_bytes - plan_bytes(a.B) - 256) / slot_bytes(sh, a.D);
   sh.slots = (int)(slots < 0 ? 0 : slots > (1 << 20) ? (1 << 20) : slots);
-  if (sh.bound <= kChunkMinPiece) sh.slots = 0;  // nothing that long: one launch
+  if (bound <= kChunkMinPiece + kChunkMergeCost) sh.slots = 0;  // nothing is cut: one launch
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   const bool f16 = a.dtype == TASFT_F16;
