@@ -1,41 +1,42 @@
 // Attention of a chunk of new tokens over a paged KV cache: how a batch is cut into tiles and
-// work items. Shared by the attention kernel and the kernel that merges split items.
+// its work shared out over the CTAs.
 #pragma once
 
 #include "common.cuh"
 
 namespace tasft {
 
-constexpr int kChunkBlk = 64;          // block size (tokens) of the kept lists
-constexpr int kChunkMaxSplits = 128;   // most items one tile is cut into
-constexpr int kChunkMinPiece = 4;      // fewest blocks an item is cut down to
-constexpr int kChunkMergeCost = 10;    // what a cut costs (partials, merge), in blocks
-constexpr int kChunkBuckets = 256;     // entries of the per-CTA prefix over sequences
+constexpr int kChunkBlk = 64;        // block size (tokens) of the kept lists
+constexpr int kChunkMinPiece = 4;    // fewest blocks a CTA's share is cut down to
+constexpr int kChunkMergeCost = 10;  // what cutting tiles costs a call (partials, merge), in blocks
+constexpr int kChunkBuckets = 256;   // entries of the per-CTA table of sequences
 
 // Launch-wide choices the host makes from types and sizes.
 struct ChunkShape {
   int mode;       // how the 128 rows of a tile are filled, see chunk_tc.cu
-  int hpt, tpt;   // query heads and tokens of a tile (mode 2: unused)
-  int units;      // tiles beside one another at the same tokens (kv-heads, or pairs of query heads)
+  int hpt, tpt;   // query heads and tokens of a tile
   int tpt_log2;   // modes 1 and 2
+  int units;      // tiles beside one another at the same tokens (kv-heads, or pairs of query heads)
   int capacity;   // tokens the block table can hold (max_pages * page_size)
-  int slots;      // split items the workspace has room for
-  int rows;       // rows of a split item's partials
-  int stride;     // sequences per entry of the per-CTA prefix
-};
-
-// Workspace: plan [B] {splits, first slot}, then (m, l) and O of every split item's rows.
-struct ChunkWs {
-  int2* plan;
-  float2* ml;   // [slots, rows] (row maximum in base-2 units, row sum)
-  float* o;     // [slots, rows, D] sums not yet divided by l
+  int rows;       // rows of a piece's partials
+  int stride;     // sequences per entry of the table
+  int may_cut;    // 0: no tile is long enough to be cut
 };
 
 struct ChunkSeq {
   int start, n, ctx, len;  // first row of its new tokens, how many, tokens before them, all tokens
   int tiles;               // per unit
+  int cost;                // blocks a tile visits, for balance alone (lists; the dense mode counts tokens)
   bool bad;
 };
+
+__device__ __forceinline__ int chunk_tiles(const ChunkShape& sh, int n, int ctx, int len) {
+  if (n <= 0) return 0;
+  if (sh.mode == 0) return (uint32_t)(n + sh.tpt - 1) / (uint32_t)sh.tpt;
+  // tiles stand at multiples of their token count, so none spans two rows of the lists (mode 2
+  // with one head per kv-head: two rows on purpose)
+  return ((len - 1) >> sh.tpt_log2) - (ctx >> sh.tpt_log2) + 1;
+}
 
 __device__ __forceinline__ ChunkSeq chunk_seq(const tasft_chunk_args& a, const ChunkShape& sh, int b) {
   ChunkSeq s;
@@ -49,39 +50,52 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const tasft_chunk_args& a, const C
     s.n = 0;
   }
   s.ctx = s.n > 0 ? s.len - s.n : 0;
-  s.tiles = 0;
-  if (s.n > 0) {
-    if (sh.mode == 0) {
-      s.tiles = (uint32_t)(s.n + sh.tpt - 1) / (uint32_t)sh.tpt;
-    } else {
-      // tiles stand at multiples of their token count, so none spans two rows of the lists
-      // (mode 2 with one head per kv-head: two rows on purpose)
-      s.tiles = ((s.len - 1) >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2) + 1;
-    }
+  s.tiles = chunk_tiles(sh, s.n, s.ctx, s.len);
+  s.cost = 0;
+  if (sh.mode != 0 && s.n > 0) {
+    // the length of the last token's list (first head; mode 2 walks two lists)
+    const int last = (s.len - 1) / kChunkBlk;
+    const int cnt = a.kept_cnt[(int64_t)b * a.Hm * a.nb_q + (last - s.ctx / kChunkBlk)];
+    s.cost = max(1, min(cnt * (sh.mode == 2 ? 2 : 1), last + 1));
   }
   return s;
 }
 
-// Blocks a tile of the sequence visits, for balance alone: those up to its last token, or the
-// length of that token's list (first head; mode 2 walks two lists).
-__device__ __forceinline__ int chunk_cost(const tasft_chunk_args& a, const ChunkShape& sh, const ChunkSeq& s, int b) {
-  if (s.n == 0) return 0;
-  const int last = (s.len - 1) / kChunkBlk;
-  if (sh.mode == 0) return last + 1;
-  const int cnt = a.kept_cnt[(int64_t)b * a.Hm * a.nb_q + (last - s.ctx / kChunkBlk)];
-  return min(max(cnt, 0) * (sh.mode == 2 ? 2 : 1), last + 1);
+// Weight of a tile (64 per block) and of all tiles of a unit before it. Without lists a tile
+// visits the blocks up to its last token; with lists all tiles of a sequence count alike.
+__device__ __forceinline__ int64_t chunk_weight(const ChunkShape& sh, const ChunkSeq& s, int i) {
+  return sh.mode == 0 ? (int64_t)s.ctx + 63 + (int64_t)(i + 1) * sh.tpt : (int64_t)s.cost * kChunkBlk;
+}
+__device__ __forceinline__ int64_t chunk_weight_before(const ChunkShape& sh, const ChunkSeq& s, int i) {
+  return sh.mode == 0 ? (int64_t)i * (s.ctx + 63) + (int64_t)sh.tpt * ((int64_t)i * (i + 1) / 2)
+                      : (int64_t)i * s.cost * kChunkBlk;
 }
 
-// Items a tile is cut into, for pieces of about `target` blocks.
-__device__ __forceinline__ int chunk_splits(int cost, int target) {
-  if (cost <= target + kChunkMergeCost) return 1;
-  return min(kChunkMaxSplits, (int)((uint32_t)(cost + target - 1) / (uint32_t)target));
-}
+// A place in the sequence of all tiles (sequence, unit, tile) and the weight `rho` into the tile;
+// b == B: the end.
+struct ChunkCut {
+  int b, unit, tile;
+  int64_t rho, w;
+  ChunkSeq s;
+};
 
-__device__ __forceinline__ int warp_scan_int(int v, int lane) {  // inclusive
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int64_t warp_max64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const int64_t x = __shfl_xor_sync(0xffffffffu, v, o);
+    v = x > v ? x : v;
+  }
+  return v;
+}
+__device__ __forceinline__ int64_t warp_scan64(int64_t v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    const int64_t t = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += t;
   }
   return v;

@@ -13,11 +13,13 @@
 //   2  lists per query head: two 64-token slots, two heads of a group at one 64-token block
 //      (one head at two blocks where a group has one head); the tile walks the union of the
 //      two lists and each entry says which slots keep it
-// A work item is a tile, or where few tiles face many blocks a slice of a tile's blocks; the
-// slices' (m, l, O) meet in chunk_merge_kernel. Every CTA computes the same cut from cu_seqlens
-// and kv_len, so the host needs neither.
-//
-// Persistent CTAs (2 per SM, 256 threads) take items in a static, snaking stride. Warps:
+// Persistent CTAs (2 per SM, 256 threads) share the work evenly: all tiles in a row, weighted by
+// the blocks they visit, are cut into as many equal lengths as there are CTAs, through the middle
+// of tiles where that gains more than the merge costs (chunk_cut). A tile cut into pieces leaves
+// each piece's (m, l, O) in the workspace and chunk_merge_kernel joins them. Every CTA computes
+// the same cuts from cu_seqlens and kv_len, so the host needs neither. A CTA takes its length from
+// the back: the piece at its end starts at block 0 and the one at its start ends at the last, so
+// CTAs that share K and V run over them side by side and find them in L2. Warps:
 //   0     producer: Q of the tile, then K and V of every entry through separate 2-stage rings
 //         (TMA from the pages, 128B swizzle)
 //   1     MMA issuer: S = Q K^T (SS, M128 N64) into a double-buffered TMEM tile, O += P V (TS:
@@ -40,6 +42,7 @@ namespace tasft {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMergeThreads = 1024;        // four rows a warp: the merge is a chain of latencies
 constexpr int kSeg = 128;                  // entries of a list segment
 constexpr uint32_t kTmemCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -99,6 +102,15 @@ struct Work {
   int pos[2];       // position of row 0 of the slot
   int row[2];       // its row in q and out (mode 2: of position pos, maybe before the sequence)
   int ctx;
+  int pieces;       // in the workspace's records: how many pieces the tile is in
+};
+
+// Workspace: one record per CTA (the tile that its length starts inside of, if it is the first to
+// do so; pieces 0 otherwise), then (m, l) and O of two pieces per CTA.
+struct ChunkWs {
+  Work* cut;
+  float2* ml;   // [2 CTAs, rows] (row maximum in base-2 units, row sum)
+  float* o;     // [2 CTAs, rows, D] sums not yet divided by l
 };
 
 template <int D>
@@ -112,9 +124,8 @@ struct Smem {
   static constexpr int kStageOff = kQOff + kQBytes;
   static constexpr int kListOff = kStageOff + 4 * kKVTileBytes;  // [2][kSeg] entries
   static constexpr int kPageOff = kListOff + 2 * kSeg * 4;       // [2][kSeg][4] pages
-  static constexpr int kItemOff = kPageOff + 2 * kSeg * 16;      // [kChunkBuckets + 1] first item
-  static constexpr int kSlotOff = kItemOff + (kChunkBuckets + 1) * 4;  // the same, first split slot
-  static constexpr int kSeqOff = (kSlotOff + (kChunkBuckets + 1) * 4 + 15) / 16 * 16;  // [kChunkBuckets] int4
+  static constexpr int kSumOff = kPageOff + 2 * kSeg * 16;        // [kChunkBuckets] int64, weight before
+  static constexpr int kSeqOff = kSumOff + kChunkBuckets * 8;     // [kChunkBuckets] int4
   static constexpr int kBitmapOff = kSeqOff + kChunkBuckets * 16;  // [2][kSeg / 32]
   static constexpr int kWorkOff = (kBitmapOff + 2 * (kSeg / 32) * 4 + 7) / 8 * 8;
   static constexpr int kBarOff = (kWorkOff + 2 * (int)sizeof(Work) + 7) / 8 * 8;
@@ -183,57 +194,36 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc::tmem_alloc(&misc[0], kTmemCols);
     tc::tmem_relinquish();
   }
-  int32_t* item0 = reinterpret_cast<int32_t*>(smem + L::kItemOff);
-  int32_t* slot0 = reinterpret_cast<int32_t*>(smem + L::kSlotOff);
-  int4* seqs = reinterpret_cast<int4*>(smem + L::kSeqOff);  // start, n, len, splits (stride 1)
-  int items = 0, target = 0;
+  int64_t* before = reinterpret_cast<int64_t*>(smem + L::kSumOff);  // weight before a bucket's first sequence
+  int4* seqs = reinterpret_cast<int4*>(smem + L::kSeqOff);          // start, n, len, cost (stride 1)
+  int64_t total = 0, step = 1;
+  bool cutting = false;
   if (warp == 2) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // ---- cut the batch into items: pieces of about the mean load of a CTA ----
-    float load = 0.f;
-    ChunkSeq s = {};
-    int cost = 0;
+    // ---- the weight of all tiles, and each CTA's length of it ----
+    int64_t widest = 0, count = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       const int b = b0 + lane;
+      int64_t w = 0;
       if (b < a.B) {
-        s = chunk_seq(a, sh, b);
-        cost = chunk_cost(a, sh, s, b);
-        load += (float)s.tiles * (float)cost;
+        const ChunkSeq s = chunk_seq(a, sh, b);
         if (s.bad && blockIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
+        w = chunk_weight_before(sh, s, s.tiles) * sh.units;
+        if (s.tiles > 0) widest = max(widest, chunk_weight(sh, s, s.tiles - 1));
+        count += s.tiles;
+        if (sh.stride == 1) seqs[b] = make_int4(s.start, s.n, s.len, s.cost);
       }
+      const int64_t upto = warp_scan64(w, lane);
+      if (b < a.B && (sh.stride == 1 || b % sh.stride == 0)) before[sh.stride == 1 ? b : b / sh.stride] = total + upto - w;
+      total += __shfl_sync(0xffffffffu, upto, 31);
     }
-    load = warp_sum(load) * (float)sh.units;
-    target = max(kChunkMinPiece, (int)ceilf(load / (float)gridDim.x));
-    int slots = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const int b = b0 + lane;
-      int it = 0, sl = 0, ns = 1;
-      if (b < a.B) {
-        if (a.B > 32) {  // else the lane's own sequence is still at hand
-          s = chunk_seq(a, sh, b);
-          cost = chunk_cost(a, sh, s, b);
-        }
-        ns = chunk_splits(cost, target);
-        it = s.tiles * sh.units;
-        sl = ns > 1 ? it * ns : 0;
-      }
-      // slots count what every sequence asks for; from the first that finds no room in the
-      // workspace on, sequences stay whole
-      const int fs = warp_scan_int(sl, lane);
-      if (slots + fs > sh.slots) ns = 1;
-      const int fi = warp_scan_int(it * ns, lane);
-      if (b < a.B) {
-        if (sh.stride == 1 || b % sh.stride == 0) {
-          const int at = sh.stride == 1 ? b : b / sh.stride;
-          item0[at] = items + fi - it * ns;
-          slot0[at] = slots + fs - sl;
-          if (sh.stride == 1) seqs[at] = make_int4(s.start, s.n, s.len, ns);
-        }
-        if (blockIdx.x == 0) ws.plan[b] = make_int2(ns, slots + fs - sl);
-      }
-      items += __shfl_sync(0xffffffffu, fi, 31);
-      slots += __shfl_sync(0xffffffffu, fs, 31);
-    }
+    widest = warp_max64(widest);
+    count = warp_sum64(count) * sh.units;
+    const int64_t G = gridDim.x;
+    step = max((total + G - 1) / G, (int64_t)kChunkMinPiece * kChunkBlk);
+    // whole tiles would take rounds * widest; cut ones take `step`
+    const int64_t rounds = (count + G - 1) / G;
+    cutting = sh.may_cut && rounds * widest - step > (int64_t)kChunkMergeCost * kChunkBlk;
     __syncwarp();
   }
   tc::tc_fence_before();
@@ -253,58 +243,114 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + L::kBitmapOff);
     const int buckets = (a.B + sh.stride - 1) / sh.stride;
     const PagedGeo geo = {max(1, kChunkBlk / a.page_size), min(kChunkBlk, a.page_size)};
+    auto get_seq = [&](int b) -> ChunkSeq {
+      if (sh.stride != 1) return chunk_seq(a, sh, b);
+      const int4 q4 = seqs[b];
+      ChunkSeq s;
+      s.start = q4.x;
+      s.n = q4.y;
+      s.len = q4.z;
+      s.cost = q4.w;
+      s.ctx = s.n > 0 ? s.len - s.n : 0;
+      s.tiles = chunk_tiles(sh, s.n, s.ctx, s.len);
+      s.bad = false;
+      return s;
+    };
+    // The place at weight x. Cuts within two blocks of a tile's end, or all where tiles stay whole,
+    // go to the nearer end.
+    auto find = [&](int64_t x) -> ChunkCut {
+      ChunkCut c;
+      c.b = a.B;
+      c.unit = c.tile = 0;
+      c.rho = 0;
+      c.w = 1;
+      if (x >= total) return c;
+      int bl = 0, bh = buckets - 1;
+      while (bl < bh) {  // the last bucket that starts at or before x
+        const int mid = (bl + bh + 1) >> 1;
+        if (before[mid] <= x) bl = mid;
+        else bh = mid - 1;
+      }
+      x -= before[bl];
+      c.b = bl * sh.stride;
+      c.s = get_seq(c.b);
+      int64_t per = chunk_weight_before(sh, c.s, c.s.tiles);
+      while (x >= per * sh.units) {  // sequences without new tokens have no weight
+        x -= per * sh.units;
+        c.s = get_seq(++c.b);
+        per = chunk_weight_before(sh, c.s, c.s.tiles);
+      }
+      c.unit = (int)(x / per);
+      x -= c.unit * per;
+      int tl = 0, th = c.s.tiles - 1;
+      while (tl < th) {
+        const int mid = (tl + th + 1) >> 1;
+        if (chunk_weight_before(sh, c.s, mid) <= x) tl = mid;
+        else th = mid - 1;
+      }
+      c.tile = tl;
+      c.rho = x - chunk_weight_before(sh, c.s, tl);
+      c.w = chunk_weight(sh, c.s, tl);
+      const int64_t edge = cutting ? 2 * kChunkBlk : (c.w + 1) / 2;
+      if (c.rho < edge) {
+        c.rho = 0;
+      } else if (c.w - c.rho < edge || !cutting) {  // the start of the next tile
+        c.rho = 0;
+        if (++c.tile == c.s.tiles) {
+          c.tile = 0;
+          if (++c.unit == sh.units) {
+            c.unit = 0;
+            do {
+              if (++c.b == a.B) break;
+              c.s = get_seq(c.b);
+            } while (c.s.tiles == 0);
+          }
+        }
+      }
+      return c;
+    };
+    const ChunkCut from = find((int64_t)blockIdx.x * step);
+    ChunkCut cur = find((int64_t)(blockIdx.x + 1) * step);
+    bool more = !(from.b == cur.b && from.unit == cur.unit && from.tile == cur.tile && from.rho == cur.rho);
+    bool partial_end = cur.rho > 0;  // the piece at hand stops inside its tile
+    // whether the CTA before this one starts inside the same tile: then that one records it
+    bool recorded = from.rho == 0;
+    if (from.rho > 0) {
+      const int64_t edge = 2 * kChunkBlk, back = from.rho - step;
+      recorded = back >= edge && blockIdx.x > 0;
+    }
+    if (recorded && lane == 0) ws.cut[blockIdx.x].pieces = 0;
 
     int u = 0;  // segment counter
     bool ok = true;
-    for (int v = 0; ok; ++v) {
-      // the CTA order snakes (0..G-1, then G-1..0, ...), heavy tiles of a sequence first
-      const int item = v * gridDim.x + ((v & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    while (ok) {
       Work w;
-      int lo = 0, hi = 0;                 // range of the item: list positions, or blocks
+      int lo = 0, hi = 0;                 // range of the piece: list positions, or blocks
       const int32_t* idx[2] = {nullptr, nullptr};
       int cnt[2] = {0, 0}, qb[2] = {0, 0};
       int b = 0;
-      const bool done = item >= items;
+      const bool done = !more;
       if (!done) {
-        int bl = 0, bh = buckets - 1;
-        while (bl < bh) {  // last bucket that starts at or before the item
-          const int mid = (bl + bh + 1) >> 1;
-          if (item0[mid] <= item) bl = mid;
-          else bh = mid - 1;
-        }
-        b = bl * sh.stride;
-        int first_item = item0[bl], first_slot = slot0[bl];
-        ChunkSeq s;
-        int ns;
-        if (sh.stride == 1) {
-          const int4 q4 = seqs[b];
-          s.start = q4.x;
-          s.n = q4.y;
-          s.len = q4.z;
-          s.ctx = s.len - s.n;
-          ns = q4.w;
-          s.tiles = sh.mode == 0 ? (int)((uint32_t)(s.n + sh.tpt - 1) / (uint32_t)sh.tpt)
-                                 : ((s.len - 1) >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2) + 1;
-        } else {
-          while (true) {
-            s = chunk_seq(a, sh, b);
-            ns = chunk_splits(chunk_cost(a, sh, s, b), target);
-            const int it = s.tiles * sh.units, ask = ns > 1 ? it * ns : 0;
-            if (first_slot + ask > sh.slots) ns = 1;
-            if (item < first_item + it * ns || b + 1 >= a.B) break;
-            first_item += it * ns;
-            first_slot += ask;
-            ++b;
+        if (!partial_end) {  // step back to the tile before
+          if (--cur.tile < 0) {
+            if (--cur.unit < 0) {
+              do {
+                cur.s = get_seq(--cur.b);
+              } while (cur.s.tiles == 0);
+              cur.unit = sh.units - 1;
+            }
+            cur.tile = cur.s.tiles - 1;
           }
         }
-        const uint32_t rest = (uint32_t)(item - first_item) / (uint32_t)sh.units;
-        const int unit = item - first_item - (int)rest * sh.units;
-        const uint32_t back = ns == 1 ? rest : rest / (uint32_t)ns;
-        const int split = (int)(rest - back * ns);
-        const int tile = s.tiles - 1 - (int)back;
+        const ChunkSeq& s = cur.s;
+        b = cur.b;
+        const int unit = cur.unit, tile = cur.tile;
+        const bool at_start = b == from.b && unit == from.unit && tile == from.tile;
+        const bool partial_start = at_start && from.rho > 0;
         w.len = s.len;
         w.ctx = s.ctx;
-        w.part = ns > 1 ? first_slot + (tile * sh.units + unit) * ns + split : -1;
+        w.part = partial_start ? 2 * (int)blockIdx.x : partial_end ? 2 * (int)blockIdx.x + 1 : -1;
+        w.pieces = 0;
         int diag;  // last block the tile may visit
         if (sh.mode == 2) {
           const int base = ((s.ctx >> sh.tpt_log2) + tile) << sh.tpt_log2;
@@ -338,8 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             cnt[x] = min(max(a.kept_cnt[lrow], 0), a.nb_w);
             idx[x] = a.kept_idx + lrow * a.nb_w;
           }
-          // (its slices are ranges of block indices)
-          lo = 0;
+          // (its pieces are ranges of block indices)
           hi = diag + 1;
         } else {
           w.hk = unit;
@@ -365,15 +410,24 @@ __global__ void __launch_bounds__(kThreads, 2)
             cnt[0] = min(max(a.kept_cnt[lrow], 0), a.nb_w);
             idx[0] = a.kept_idx + lrow * a.nb_w;
           }
-          lo = 0;
           hi = cnt[0];
         }
-        if (ns > 1) {  // at most 2^20 blocks in 2^7 slices
-          lo = (int)((uint32_t)(split * hi) / (uint32_t)ns);
-          hi = (int)((uint32_t)((split + 1) * hi) / (uint32_t)ns);
+        // the cuts' places in the tile: both CTAs beside a cut compute the same one
+        const int all = hi;
+        if (partial_end) hi = (int)((uint64_t)(cur.rho * all) / (uint64_t)cur.w);
+        if (partial_start) lo = (int)((uint64_t)(from.rho * all) / (uint64_t)from.w);
+        if (partial_start && !recorded) {
+          // pieces: the CTA before, this one, and those that start further on in the tile
+          if (lane == 0) {
+            w.pieces = 2 + (int)((from.w - 2 * kChunkBlk - from.rho) / step);
+            ws.cut[blockIdx.x] = w;
+            w.pieces = 0;
+          }
         }
+        partial_end = false;
+        more = !at_start;
       }
-      // ---- the item's segments ----
+      // ---- the piece's segments ----
       int at = lo;                       // next list position or block
       int pt[2] = {0, 0};                // mode 2: next position of each list
       int prev[2] = {-1, -1};            // last accepted block of each list
@@ -837,74 +891,117 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// Rows of split items: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, splits in order.
-// One warp per (token, query head); D / 32 consecutive columns per lane.
+// Tiles in pieces: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, pieces in order. CTA c
+// joins the tile that work CTA c was the first to start inside of: its pieces are the second
+// partial of CTA c - 1 and the first ones of CTAs c, c + 1, ... A warp takes a row at a time; lane
+// x holds piece x's weight; D / 32 consecutive columns per lane, eight pieces' loads in flight.
 template <int D, bool kF16>
-__global__ void __launch_bounds__(256) chunk_merge_kernel(const tasft_chunk_args a, const ChunkShape sh, const ChunkWs ws) {
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const tasft_chunk_args a, const ChunkShape sh, const ChunkWs ws) {
   using T = typename std::conditional<kF16, __half, __nv_bfloat16>::type;
   constexpr int V = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int grp = a.Hq / a.Hk;
-  const int64_t rows = (int64_t)a.T * a.Hq;
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < rows;
-       i += (int64_t)gridDim.x * (blockDim.x >> 5)) {
-    const int t = (int)(i / a.Hq), head = (int)(i % a.Hq);
-    int bl = 0, bh = a.B - 1;
-    while (bl < bh) {  // last sequence that starts at or before the token (empty ones share a start)
-      const int mid = (bl + bh + 1) >> 1;
-      if (a.cu_seqlens[mid] <= t) bl = mid;
-      else bh = mid - 1;
-    }
-    const ChunkSeq s = chunk_seq(a, sh, bl);
-    if (s.n == 0 || t < s.start || t >= s.start + s.n) continue;
-    const int2 plan = ws.plan[bl];
-    const int ns = plan.x;
-    if (ns <= 1) continue;
-    const int pos = s.ctx + t - s.start, hk = head / grp, hg = head % grp;
-    int tile, unit, row;
-    if (sh.mode == 2) {
-      tile = (pos >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2);
-      unit = grp >= 2 ? hk * ((grp + 1) / 2) + hg / 2 : hk;
-      row = grp >= 2 ? (hg & 1) * 64 + (pos & 63) : pos & 127;
-    } else {
-      unit = hk;
-      if (sh.mode == 0) {
-        tile = (t - s.start) / sh.tpt;
-        row = (t - s.start - tile * sh.tpt) * sh.hpt + hg;
-      } else {
-        tile = (pos >> sh.tpt_log2) - (s.ctx >> sh.tpt_log2);
-        row = (pos - max(s.ctx, pos >> sh.tpt_log2 << sh.tpt_log2)) * sh.hpt + hg;
-      }
-    }
-    const int64_t part = plan.y + (int64_t)(tile * sh.units + unit) * ns;
-    // lane x holds slice x's weight; the slices' O, eight loads in flight, are added in order
-    float M = -INFINITY;
-    for (int x = lane; x < ns; x += 32) M = fmaxf(M, ws.ml[(part + x) * sh.rows + row].x);
-    M = warp_max(M);
-    float acc[V], sum = 0.f;
+  const int c = blockIdx.x;
+  const Work w = ws.cut[c];
+  const int ns = w.pieces;
+  if (ns == 0) return;
+  const int warp = threadIdx.x >> 5;
+  // where a row of the tile goes, or null
+  auto target = [&](int r) -> T* {
+    const int slot = sh.mode == 2 ? r >> 6 : 0;
+    const int tok = sh.mode == 2 ? r & 63 : r / sh.hpt;
+    const int hd = sh.mode == 2 ? 0 : r % sh.hpt;
+    const int qpos = (slot ? w.pos[1] : w.pos[0]) + tok;
+    const bool live = sh.mode == 2 ? (slot ? w.valid[1] : w.valid[0]) && qpos >= w.ctx && qpos < w.len : tok < w.valid[0];
+    if (r >= sh.rows || !live) return nullptr;
+    return reinterpret_cast<T*>(a.out) + (int64_t)((slot ? w.row[1] : w.row[0]) + tok) * a.o_stride[0] +
+           (int64_t)((slot ? w.head[1] : w.head[0]) + hd) * a.o_stride[1] + lane * V;
+  };
+  auto place = [&](int x) -> int64_t { return (int64_t)(x == 0 ? 2 * c - 1 : 2 * (c + x - 1)) * sh.rows; };
+  auto store = [&](T* dst, const float* acc, float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint32_t pk[V / 2];
 #pragma unroll
-    for (int c = 0; c < V; ++c) acc[c] = 0.f;
-    for (int x0 = 0; x0 < ns; x0 += 32) {
-      float wgt = 0.f, lw = 0.f;
-      if (x0 + lane < ns) {
-        const float2 ml = ws.ml[(part + x0 + lane) * sh.rows + row];
-        if (ml.y != 0.f) {  // a slice with nothing to see wrote no O
-          wgt = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
-          lw = wgt * ml.y;
+    for (int i = 0; i < V / 2; ++i)
+      pk[i] = kF16 ? tc::pack_f16x2(acc[2 * i] * inv, acc[2 * i + 1] * inv)
+                   : tc::pack_bf16x2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pk[0], pk[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = pk[0];
+  };
+  if (ns <= 8) {
+    // many rows, few pieces: a warp's four rows at once, eight lanes on the pieces of each
+    const int mine = lane >> 3, x = lane & 7, r0 = warp + mine * 32;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (x < ns && r0 < sh.rows && target(r0)) ml = ws.ml[place(x) + r0];
+    float M = ml.x;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float wgt = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
+    float sum = wgt * ml.y;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const unsigned have = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    float acc[4][V];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[i][k] = 0.f;
+    for (int p = 0; p < ns; ++p) {
+      float v[4][V];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[i][k] = 0.f;
+        if ((have >> (8 * i + p)) & 1) {
+          const float* o = ws.o + (place(p) + warp + 32 * i) * D + lane * V;
+          if constexpr (V == 4) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(o);
+          else *reinterpret_cast<float2*>(v[i]) = *reinterpret_cast<const float2*>(o);
         }
       }
-      const unsigned have = __ballot_sync(0xffffffffu, lw != 0.f || wgt != 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float wp = __shfl_sync(0xffffffffu, wgt, 8 * i + p);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[i][k] += wp * v[i][k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float total = __shfl_sync(0xffffffffu, sum, 8 * i);
+      if (T* dst = target(warp + 32 * i)) store(dst, acc[i], total);
+    }
+    return;
+  }
+  for (int r = warp; r < sh.rows; r += kMergeThreads / 32) {
+    T* dst = target(r);
+    if (!dst) continue;
+    float M = -INFINITY, acc[V], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int x0 = 0; x0 < ns; x0 += 32) {
       const int nx = min(32, ns - x0);
+      const float2 ml = lane < nx ? ws.ml[place(x0 + lane) + r] : make_float2(-INFINITY, 0.f);
+      const float Mn = fmaxf(M, warp_max(ml.x));
+      if (Mn != M) {  // earlier pieces (more than 32) move to the new maximum
+        const float f = M == -INFINITY ? 1.f : ex2(M - Mn);
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] *= f;
+        M = Mn;
+      }
+      // a piece with nothing to see (l = 0) wrote no O
+      const float wgt = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
+      const unsigned have = __ballot_sync(0xffffffffu, ml.y != 0.f);
+      const float lw = wgt * ml.y;
       for (int x1 = 0; x1 < nx; x1 += 8) {
         float v[8][V];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
 #pragma unroll
-          for (int c = 0; c < V; ++c) v[x][c] = 0.f;
-          if (x1 + x < nx && ((have >> (x1 + x)) & 1)) {
-            const float* o = ws.o + ((part + x0 + x1 + x) * sh.rows + row) * D + lane * V;
+          for (int i = 0; i < V; ++i) v[x][i] = 0.f;
+          if ((have >> (x1 + x)) & 1) {
+            const float* o = ws.o + (place(x0 + x1 + x) + r) * D + lane * V;
             if constexpr (V == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(o);
             else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(o);
           }
@@ -912,22 +1009,14 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const tasft_chunk_args
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           if (x1 + x >= nx) break;
-          const float w = __shfl_sync(0xffffffffu, wgt, x1 + x);
+          const float wx = __shfl_sync(0xffffffffu, wgt, x1 + x);
           sum += __shfl_sync(0xffffffffu, lw, x1 + x);
 #pragma unroll
-          for (int c = 0; c < V; ++c) acc[c] += w * v[x][c];
+          for (int i = 0; i < V; ++i) acc[i] += wx * v[x][i];
         }
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* orow = reinterpret_cast<T*>(a.out) + (int64_t)t * a.o_stride[0] + (int64_t)head * a.o_stride[1] + lane * V;
-    uint32_t pk[V / 2];
-#pragma unroll
-    for (int c = 0; c < V / 2; ++c)
-      pk[c] = kF16 ? tc::pack_f16x2(acc[2 * c] * inv, acc[2 * c + 1] * inv)
-                   : tc::pack_bf16x2(acc[2 * c] * inv, acc[2 * c + 1] * inv);
-    if constexpr (V == 4) *reinterpret_cast<uint2*>(orow) = make_uint2(pk[0], pk[1]);
-    else *reinterpret_cast<uint32_t*>(orow) = pk[0];
+    store(dst, acc, sum);
   }
 }
 
@@ -958,8 +1047,17 @@ bool chunk_shape(ChunkShape& sh, int Hq, int Hk, int Hm, int max_q) {
   return true;
 }
 
-int64_t plan_bytes(int B) { return ((int64_t)B * 8 + 255) / 256 * 256; }
-int64_t slot_bytes(const ChunkShape& sh, int D) { return (int64_t)sh.rows * (D + 2) * 4; }
+// Parts of the workspace for G work CTAs, in bytes from its start.
+struct WsLayout {
+  int64_t ml, o, bytes;
+};
+WsLayout ws_layout(const ChunkShape& sh, int D, int G) {
+  WsLayout w;
+  w.ml = ((int64_t)G * sizeof(Work) + 255) / 256 * 256;
+  w.o = w.ml + (2LL * G * sh.rows * 8 + 255) / 256 * 256;
+  w.bytes = w.o + 2LL * G * sh.rows * D * 4;
+  return w;
+}
 
 template <int D, bool kF16>
 int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
@@ -974,13 +1072,12 @@ int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
   const int smem = Smem<D>::kAlloc;
   static std::atomic<uint64_t> allowed{0};
   if (!allow_smem(kern, smem, allowed)) return TASFT_ERR_CUDA;
-  ChunkWs ws;
-  uint8_t* p = reinterpret_cast<uint8_t*>(a.workspace);
-  ws.plan = reinterpret_cast<int2*>(p);
-  ws.ml = reinterpret_cast<float2*>(p + plan_bytes(a.B));
-  ws.o = reinterpret_cast<float*>(p + plan_bytes(a.B) + ((int64_t)sh.slots * sh.rows * 8 + 255) / 256 * 256);
   const int grid = 2 * sms;  // persistent: two CTAs per SM
-  if (debug_enabled()) debug_log("chunk_tc D=%d mode=%d grid=%d slots=%d smem=%d", D, sh.mode, grid, sh.slots, smem);
+  const WsLayout lay = ws_layout(sh, D, grid);
+  uint8_t* p = reinterpret_cast<uint8_t*>(a.workspace);
+  const ChunkWs ws = {reinterpret_cast<Work*>(p), reinterpret_cast<float2*>(p + lay.ml),
+                      reinterpret_cast<float*>(p + lay.o)};
+  if (debug_enabled()) debug_log("chunk_tc D=%d mode=%d grid=%d smem=%d", D, sh.mode, grid, smem);
   // both launches may begin while the kernel before them ends; they wait for it on the device
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -994,10 +1091,8 @@ int launch(const tasft_chunk_args& a, ChunkShape sh, int sms, cudaStream_t st) {
   cfg.numAttrs = 1;
   int rc = cuda_status(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, a, sh, ws));
   count_launch();
-  if (rc != TASFT_OK || sh.slots == 0) return rc;
-  const int64_t rows = (int64_t)a.T * a.Hq;
-  cfg.gridDim = dim3((unsigned)(rows / 8 + 1 < 4LL * sms ? rows / 8 + 1 : 4LL * sms));
-  cfg.blockDim = dim3(256);
+  if (rc != TASFT_OK || !sh.may_cut) return rc;
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.dynamicSmemBytes = 0;
   rc = cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<D, kF16>, a, sh, ws));
   count_launch();
@@ -1014,12 +1109,7 @@ extern "C" int64_t tasft_chunk_workspace_size(int32_t B, int32_t T, int32_t Hq, 
   if (B <= 0 || T < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D <= 0 || max_q <= 0 || Hm < 0) return TASFT_ERR_INVALID_ARG;
   ChunkShape sh;
   if (!chunk_shape(sh, Hq, Hk, Hm, max_q)) return TASFT_ERR_UNSUPPORTED;
-  // Pieces hold at least a CTA's mean load, so split tiles make at most twice as many pieces as
-  // there are CTAs; and a tile makes at most kChunkMaxSplits.
-  const int64_t tiles = ((int64_t)T / sh.tpt + 2LL * B) * sh.units;
-  int64_t slots = 4LL * sm_count();
-  if (tiles * kChunkMaxSplits < slots) slots = tiles * kChunkMaxSplits;
-  return plan_bytes(B) + slots * slot_bytes(sh, D) + 256;
+  return ws_layout(sh, D, 2 * sm_count()).bytes;
 }
 
 extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_stream_t stream) {
@@ -1055,10 +1145,8 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   int bound = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
   if (a.kept_idx && (int64_t)a.nb_w * 2 < bound) bound = a.nb_w * (sh.mode == 2 ? 2 : 1);
   sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
-  if (!a.workspace || a.workspace_bytes < plan_bytes(a.B)) return TASFT_ERR_WORKSPACE;
-  const int64_t slots = (a.workspace_bytes - plan_bytes(a.B) - 256) / slot_bytes(sh, a.D);
-  sh.slots = (int)(slots < 0 ? 0 : slots > (1 << 20) ? (1 << 20) : slots);
-  if (bound <= kChunkMinPiece + kChunkMergeCost) sh.slots = 0;  // nothing is cut: one launch
+  sh.may_cut = bound > kChunkMergeCost;  // else one launch
+  if (!a.workspace || a.workspace_bytes < ws_layout(sh, a.D, 2 * sm_count()).bytes) return TASFT_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   const bool f16 = a.dtype == TASFT_F16;
