@@ -194,6 +194,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc::tmem_alloc(&misc[0], kTmemCols);
     tc::tmem_relinquish();
   }
+  if (warp == 3) {
+    // tables and lists, a share per CTA, on their way to L2 while warp 2 counts: it reads them in
+    // a chain (a prefetch of what the kernel before is still writing does no harm, L2 holds it)
+    auto fetch = [&](const void* p, int64_t bytes) {
+      const int64_t lines = (bytes + 127) / 128, stride = (int64_t)gridDim.x * 32;
+      for (int64_t i = (int64_t)blockIdx.x * 32 + lane, k = 0; i < lines && k < 4; i += stride, ++k)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p) + i * 128));
+    };
+    fetch(a.block_table, (int64_t)a.B * a.max_pages * 4);
+    if (a.kept_idx) {
+      fetch(a.kept_cnt, (int64_t)a.B * a.Hm * a.nb_q * 4);
+      fetch(a.kept_idx, (int64_t)a.B * a.Hm * a.nb_q * a.nb_w * 4);
+    }
+  }
   int64_t* before = reinterpret_cast<int64_t*>(smem + L::kSumOff);  // weight before a bucket's first sequence
   int4* seqs = reinterpret_cast<int4*>(smem + L::kSeqOff);          // start, n, len, cost (stride 1)
   int64_t total = 0, step = 1;
@@ -220,9 +234,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     widest = warp_max64(widest);
     count = warp_sum64(count) * sh.units;
     const int64_t G = gridDim.x;
-    step = max((total + G - 1) / G, (int64_t)kChunkMinPiece * kChunkBlk);
+    step = total + G < (1ll << 32) ? (uint32_t)(total + G - 1) / (uint32_t)G : (total + G - 1) / G;
+    step = max(step, (int64_t)kChunkMinPiece * kChunkBlk);
     // whole tiles would take rounds * widest; cut ones take `step`
-    const int64_t rounds = (count + G - 1) / G;
+    const int64_t rounds = (uint32_t)(count + G - 1) / (uint32_t)G;
     cutting = sh.may_cut && rounds * widest - step > (int64_t)kChunkMergeCost * kChunkBlk;
     __syncwarp();
   }
@@ -242,7 +257,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + L::kBitmapOff);
     const int buckets = (a.B + sh.stride - 1) / sh.stride;
-    const PagedGeo geo = {max(1, kChunkBlk / a.page_size), min(kChunkBlk, a.page_size)};
+    const int page_log2 = 31 - __clz(a.page_size);
+    const PagedGeo geo = {max(1, kChunkBlk >> page_log2), min(kChunkBlk, a.page_size)};
     auto get_seq = [&](int b) -> ChunkSeq {
       if (sh.stride != 1) return chunk_seq(a, sh, b);
       const int4 q4 = seqs[b];
@@ -256,41 +272,45 @@ __global__ void __launch_bounds__(kThreads, 2)
       s.bad = false;
       return s;
     };
-    // The place at weight x. Cuts within two blocks of a tile's end, or all where tiles stay whole,
-    // go to the nearer end.
-    auto find = [&](int64_t x) -> ChunkCut {
+    // The place at weight x, in Int arithmetic. Cuts within two blocks of a tile's end, or all
+    // where tiles stay whole, go to the nearer end.
+    auto find = [&](auto zero, int64_t x64) -> ChunkCut {
+      using Int = decltype(zero);
       ChunkCut c;
       c.b = a.B;
       c.unit = c.tile = 0;
       c.rho = 0;
       c.w = 1;
-      if (x >= total) return c;
+      if (x64 >= total) return c;
       int bl = 0, bh = buckets - 1;
       while (bl < bh) {  // the last bucket that starts at or before x
         const int mid = (bl + bh + 1) >> 1;
-        if (before[mid] <= x) bl = mid;
+        if (before[mid] <= x64) bl = mid;
         else bh = mid - 1;
       }
-      x -= before[bl];
+      Int x = (Int)(x64 - before[bl]);
       c.b = bl * sh.stride;
       c.s = get_seq(c.b);
-      int64_t per = chunk_weight_before(sh, c.s, c.s.tiles);
-      while (x >= per * sh.units) {  // sequences without new tokens have no weight
-        x -= per * sh.units;
+      Int per = (Int)chunk_weight_before(sh, c.s, c.s.tiles);
+      while (x >= per * (Int)sh.units) {  // sequences without new tokens have no weight
+        x -= per * (Int)sh.units;
         c.s = get_seq(++c.b);
-        per = chunk_weight_before(sh, c.s, c.s.tiles);
+        per = (Int)chunk_weight_before(sh, c.s, c.s.tiles);
       }
       c.unit = (int)(x / per);
-      x -= c.unit * per;
-      int tl = 0, th = c.s.tiles - 1;
-      while (tl < th) {
-        const int mid = (tl + th + 1) >> 1;
-        if (chunk_weight_before(sh, c.s, mid) <= x) tl = mid;
-        else th = mid - 1;
+      x -= (Int)c.unit * per;
+      if (sh.mode != 0) {
+        c.tile = (int)(x / (Int)(c.s.cost * kChunkBlk));
+      } else {  // the weights before tiles grow as t i^2 / 2 + (ctx + 63 + t / 2) i
+        const float t = (float)sh.tpt, h = (float)(c.s.ctx + 63) + 0.5f * t;
+        int i = (int)((sqrtf(h * h + 2.f * t * (float)x) - h) / t);
+        i = max(0, min(i, c.s.tiles - 1));
+        while (i > 0 && (Int)chunk_weight_before(sh, c.s, i) > x) --i;
+        while (i + 1 < c.s.tiles && (Int)chunk_weight_before(sh, c.s, i + 1) <= x) ++i;
+        c.tile = i;
       }
-      c.tile = tl;
-      c.rho = x - chunk_weight_before(sh, c.s, tl);
-      c.w = chunk_weight(sh, c.s, tl);
+      c.rho = (int64_t)(x - (Int)chunk_weight_before(sh, c.s, c.tile));
+      c.w = chunk_weight(sh, c.s, c.tile);
       const int64_t edge = cutting ? 2 * kChunkBlk : (c.w + 1) / 2;
       if (c.rho < edge) {
         c.rho = 0;
@@ -309,8 +329,21 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       return c;
     };
-    const ChunkCut from = find((int64_t)blockIdx.x * step);
-    ChunkCut cur = find((int64_t)(blockIdx.x + 1) * step);
+    // both ends at once, in the even and the odd lanes
+    const int64_t end_x = (int64_t)(blockIdx.x + (lane & 1)) * step;
+    const ChunkCut end = total < (1ll << 31) ? find(0u, end_x) : find((int64_t)0, end_x);
+    auto take = [&](int from_lane) -> ChunkCut {
+      ChunkCut c;
+      c.b = __shfl_sync(0xffffffffu, end.b, from_lane);
+      c.unit = __shfl_sync(0xffffffffu, end.unit, from_lane);
+      c.tile = __shfl_sync(0xffffffffu, end.tile, from_lane);
+      c.rho = __shfl_sync(0xffffffffu, end.rho, from_lane);
+      c.w = __shfl_sync(0xffffffffu, end.w, from_lane);
+      return c;
+    };
+    const ChunkCut from = take(0);
+    ChunkCut cur = take(1);
+    if (cur.b < a.B) cur.s = get_seq(cur.b);
     bool more = !(from.b == cur.b && from.unit == cur.unit && from.tile == cur.tile && from.rho == cur.rho);
     bool partial_end = cur.rho > 0;  // the piece at hand stops inside its tile
     // whether the CTA before this one starts inside the same tile: then that one records it
@@ -414,8 +447,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         // the cuts' places in the tile: both CTAs beside a cut compute the same one
         const int all = hi;
-        if (partial_end) hi = (int)((uint64_t)(cur.rho * all) / (uint64_t)cur.w);
-        if (partial_start) lo = (int)((uint64_t)(from.rho * all) / (uint64_t)from.w);
+        auto part_of = [&](int64_t rho, int64_t wt) -> int {
+          const uint64_t x = (uint64_t)(rho * all);
+          return (x >> 32) == 0 ? (int)((uint32_t)x / (uint32_t)wt) : (int)(x / (uint64_t)wt);
+        };
+        if (partial_end) hi = part_of(cur.rho, cur.w);
+        if (partial_start) lo = part_of(from.rho, from.w);
         if (partial_start && !recorded) {
           // pieces: the CTA before, this one, and those that start further on in the tile
           if (lane == 0) {
@@ -517,21 +554,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         // ---- their pages ----
         for (int i = lane; i < n; i += 32) {
           const int e = list[i], kb = e & kKbMask;
+          // kv_len is within the table's capacity, so the pages of its tokens have entries
+          const int32_t* row = a.block_table + (int64_t)b * a.max_pages + (kb * kChunkBlk >> page_log2);
           int pg[4] = {0, 0, 0, 0}, have = 0;
-          const int32_t* row = a.block_table + (int64_t)b * a.max_pages;
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (x < geo.nsub && kb * kChunkBlk + x * geo.sub_rows < w.len) pg[x] = row[x];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            if (x >= geo.nsub) break;
-            const int tok = kb * kChunkBlk + x * geo.sub_rows;
-            if (tok < w.len) {  // kv_len is within the table's capacity
-              const int p = row[tok / a.page_size];
-              if (p >= 0 && p < a.num_pages) {
-                pg[x] = p;
-                have |= 1 << x;
-              } else {
-                set_err(a.err, TASFT_DEVERR_INDEX);
-              }
-            }
+            if (x >= geo.nsub || kb * kChunkBlk + x * geo.sub_rows >= w.len) continue;
+            if (pg[x] >= 0 && pg[x] < a.num_pages) have |= 1 << x;
+            else set_err(a.err, TASFT_DEVERR_INDEX);
           }
           list[i] = e | (have << kKbBits);
           pgs[i] = make_int4(pg[0], pg[1], pg[2], pg[3]);
