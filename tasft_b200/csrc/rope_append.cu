@@ -13,16 +13,17 @@
 // they are held, divided by the block. A key block begun by an earlier call is read back from
 // the cache, so its mean depends only on what the cache holds.
 //
-// Bound by HBM: every row is read and written once. One CTA of 8 warps takes one 64-token block
-// of one sequence and a share of its heads; a warp takes a head at a time, lanes over
-// (16-byte column pairs x rows), and holds the block sums in registers.
+// Bound by HBM: every row is read and written once. One CTA of 4 warps takes one 64-token block
+// of one sequence and as many of its heads; a warp takes a head, lanes over (16-byte column
+// pairs x rows), and holds the block sums in registers.
 #include "common.cuh"
 
 namespace tasft {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;  // one head per warp
 constexpr int kRopeBlk = 64;
+constexpr int kRopeRows = 64;      // rows whose cos and sin are at hand at a time (16 and 32 were slower)
 
 template <typename T>
 __device__ __forceinline__ void pack16(uint4& u, const float* f);
@@ -81,12 +82,13 @@ __device__ __forceinline__ void add_pair(float* acc, const uint4& u1, const uint
 }
 
 template <typename T, bool kMixed>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const tasft_rope_append_args a) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasft_rope_append_args a) {
   constexpr int V = Vec16<T>::N;
-  extern __shared__ float trig[];  // [rows of the block][rot / 2] cos, then sin
+  // [row][float4 of cos, then of sin][column pair]: the lanes of a row read 16 bytes beside one another
+  extern __shared__ __align__(16) float trig[];
   __shared__ int64_t place[kRopeBlk];  // element offset of each row in the page pools; -1: not there
   __shared__ int64_t place_v[kRopeBlk];
-  const int b = blockIdx.y, qi = blockIdx.x;
+  const int b = blockIdx.z, qi = blockIdx.y;  // heads vary fastest: a block's rows are read together
   const int half = a.rot / 2;
   const int start = a.cu_seqlens[b], end = a.cu_seqlens[b + 1], len = a.kv_len[b];
   const int n = end - start;
@@ -97,17 +99,15 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const tasft_r
   const bool there = !bad && n > 0 && (int64_t)blk * kRopeBlk < len;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = a.Hq + 2 * a.Hk;
-  const int h_lo = (int)((int64_t)blockIdx.z * heads / gridDim.z), h_hi = (int)((int64_t)(blockIdx.z + 1) * heads / gridDim.z);
+  const int h = blockIdx.x * (kRopeThreads / 32) + warp;
   if (!there) {
-    if (bad && qi == 0 && blockIdx.z == 0 && threadIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
-    if (a.pooled_q)  // a row that no new token falls in has a mean of zero
-      for (int h = h_lo + warp; h < min(h_hi, a.Hq); h += kRopeThreads / 32)
-        for (int d = lane; d < a.D; d += 32) a.pooled_q[(((int64_t)b * a.Hq + h) * a.NBq + qi) * a.D + d] = 0.f;
+    if (bad && qi == 0 && blockIdx.x == 0 && threadIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
+    if (a.pooled_q && h < a.Hq)  // a row that no new token falls in has a mean of zero
+      for (int d = lane; d < a.D; d += 32) a.pooled_q[(((int64_t)b * a.Hq + h) * a.NBq + qi) * a.D + d] = 0.f;
     return;
   }
   const int p0 = blk * kRopeBlk;
   const int r_lo = max(ctx - p0, 0), r_hi = min(len - p0, kRopeBlk);  // rows of the block with new tokens
-  const int nrow = r_hi - r_lo;
 
   // ---- where the block's rows lie ----
   if (threadIdx.x < kRopeBlk) {
@@ -118,129 +118,140 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const tasft_r
       if (pg >= 0 && pg < a.num_pages) {
         at = pg * a.k_stride[0] + (p % a.page_size) * a.k_stride[1];
         atv = pg * a.v_stride[0] + (p % a.page_size) * a.v_stride[1];
-      } else if (blockIdx.z == 0) {
+      } else if (blockIdx.x == 0) {
         set_err(a.err, TASFT_DEVERR_INDEX);
       }
     }
     place[r] = at;
     place_v[r] = atv;
   }
-  // ---- cos and sin of the new rows: a thread steps one pair through a segment of rows ----
-  float* cs = trig;
-  float* sn = trig + kRopeBlk * half;
-  if (half > 0 && h_lo < a.Hq + a.Hk) {
-    const int segs = max(1, kRopeThreads / half), per = (nrow + segs - 1) / segs;
-    for (int w = threadIdx.x; w < segs * half; w += kRopeThreads) {
-      const int i = w % half, seg = w / half;
-      const int first = seg * per, lastr = min(first + per, nrow);
-      if (first >= lastr) continue;
-      const double f = (a.freq_f64 ? reinterpret_cast<const double*>(a.inv_freq)[i]
-                                   : (double)reinterpret_cast<const float*>(a.inv_freq)[i]) *
-                       0.15915494309189533577;  // turns per position
-      double turns = (double)(p0 + r_lo + first) * f;
-      turns -= rint(turns);
-      double s, c, ds, dc;
-      sincospi(2.0 * turns, &s, &c);
-      if (lastr - first > 1) sincospi(2.0 * (f - rint(f)), &ds, &dc);
-      for (int r = first; r < lastr; ++r) {
-        cs[r * half + i] = (float)(c * a.factor);
-        sn[r * half + i] = (float)(s * a.factor);
-        if (r + 1 < lastr) {
-          const double c2 = c * dc - s * ds;
-          s = s * dc + c * ds;
-          c = c2;
-        }
-      }
-    }
-  }
-  __syncthreads();
-
-  // ---- heads: lanes over (column pair, row) ----
+  constexpr int kQuads = 2 * V / 4;    // float4s of cos and sin that a column pair takes
+  const int turned = a.rot / (2 * V);  // column pairs of a row that turn
+  // ---- the warp's head: lanes over (column pair, row) ----
   const int items = a.D / (2 * V);     // 16-byte column pairs of a row, at most 32
   const int step = 32 / items;         // rows at once
   const int item = lane % items, r0 = lane / items;
-  const bool active = r0 < step;       // lanes left over where items does not divide 32
-  const int turned = a.rot / (2 * V);  // of the pairs, rotated
-  for (int h = h_lo + warp; h < h_hi; h += kRopeThreads / 32) {
-    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
-    const int hh = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
-    const bool rotated = !is_v && item < turned;
-    // columns of the pair: half layout (i, i + rot/2), otherwise neighbours
-    const int c1 = !kMixed && rotated ? item * V : 2 * item * V;
-    const int c2 = !kMixed && rotated ? item * V + half : (2 * item + 1) * V;
-    const int64_t in_step = is_q ? a.q_stride[0] : is_v ? a.v_in_stride[0] : a.k_in_stride[0];
-    const int64_t in_head = is_q ? a.q_stride[1] : is_v ? a.v_in_stride[1] : a.k_in_stride[1];
-    const int64_t tok0 = (int64_t)start + p0 - ctx;  // token of the block's row 0
-    const T* in = reinterpret_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + hh * in_head + tok0 * in_step;
-    T* out;
-    if (is_q) out = reinterpret_cast<T*>(a.q_out) + hh * a.o_stride[1] + tok0 * a.o_stride[0];
-    else if (is_v) out = reinterpret_cast<T*>(a.v_pages) + hh * a.v_stride[2];
-    else out = reinterpret_cast<T*>(a.k_pages) + hh * a.k_stride[2];
-    const int64_t* at = is_v ? place_v : place;
-    const bool sum = is_q ? a.pooled_q != nullptr : !is_v && a.pooled_k != nullptr && blk < a.NBk;
-    float acc[2 * V];
+  const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
+  // (lanes left over where items does not divide 32, and warps behind the last head, do nothing)
+  const bool active = r0 < step && h < heads;
+  const int hh = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
+  const bool rotated = !is_v && item < turned;
+  // columns of the pair: half layout (i, i + rot/2), otherwise neighbours
+  const int c1 = !kMixed && rotated ? item * V : 2 * item * V;
+  const int c2 = !kMixed && rotated ? item * V + half : (2 * item + 1) * V;
+  const int64_t in_step = is_q ? a.q_stride[0] : is_v ? a.v_in_stride[0] : a.k_in_stride[0];
+  const int64_t in_head = is_q ? a.q_stride[1] : is_v ? a.v_in_stride[1] : a.k_in_stride[1];
+  const int64_t tok0 = (int64_t)start + p0 - ctx;  // token of the block's row 0
+  const T* in = reinterpret_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + hh * in_head + tok0 * in_step;
+  T* out;
+  if (is_q) out = reinterpret_cast<T*>(a.q_out) + hh * a.o_stride[1] + tok0 * a.o_stride[0];
+  else if (is_v) out = reinterpret_cast<T*>(a.v_pages) + hh * a.v_stride[2];
+  else out = reinterpret_cast<T*>(a.k_pages) + hh * a.k_stride[2];
+  const int64_t* at = is_v ? place_v : place;
+  const bool sum = is_q ? a.pooled_q != nullptr : !is_v && a.pooled_k != nullptr && blk < a.NBk;
+  float acc[2 * V];
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) acc[i] = 0.f;
-    // rows go kBatch at a time, every load of a batch before its first store
-    constexpr int kBatch = 4;
-    if (active && sum && !is_q) {  // key rows of earlier calls
-      for (int rb = r0; rb < r_lo; rb += kBatch * step) {
-        uint4 u1[kBatch], u2[kBatch];
+  for (int i = 0; i < 2 * V; ++i) acc[i] = 0.f;
+  // rows go kBatch at a time, every load of a batch before its first store
+  constexpr int kBatch = 4;
+  __syncthreads();
+  if (active && sum && !is_q) {  // key rows of earlier calls
+    for (int rb = r0; rb < r_lo; rb += kBatch * step) {
+      uint4 u1[kBatch], u2[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int r = rb + i * step;
-          u1[i] = u2[i] = make_uint4(0, 0, 0, 0);
-          if (r < r_lo && at[r] >= 0) {
-            u1[i] = *reinterpret_cast<const uint4*>(out + at[r] + c1);
-            u2[i] = *reinterpret_cast<const uint4*>(out + at[r] + c2);
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = rb + i * step;
+        u1[i] = u2[i] = make_uint4(0, 0, 0, 0);
+        if (r < r_lo && at[r] >= 0) {
+          u1[i] = *reinterpret_cast<const uint4*>(out + at[r] + c1);
+          u2[i] = *reinterpret_cast<const uint4*>(out + at[r] + c2);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) add_pair<T>(acc, u1[i], u2[i]);
+    }
+  }
+  const bool any_turn = half > 0 && blockIdx.x * (kRopeThreads / 32) < a.Hq + a.Hk;
+  for (int lo = r_lo; lo < r_hi; lo = (lo / kRopeRows + 1) * kRopeRows) {
+    const int hi = min((lo / kRopeRows + 1) * kRopeRows, r_hi);
+    // ---- cos and sin of the rows: a thread steps one pair through a segment of them ----
+    if (any_turn) {
+      if (lo > r_lo) __syncthreads();  // the rows before are done with theirs
+      const int segs = max(1, kRopeThreads / half), per = (hi - lo + segs - 1) / segs;
+      for (int w = threadIdx.x; w < segs * half; w += kRopeThreads) {
+        const int i = w % half, seg = w / half, e = i % V;
+        const int first = seg * per, lastr = min(first + per, hi - lo);
+        if (first >= lastr) continue;
+        const double f = (a.freq_f64 ? reinterpret_cast<const double*>(a.inv_freq)[i]
+                                     : (double)reinterpret_cast<const float*>(a.inv_freq)[i]) *
+                         0.15915494309189533577;  // turns per position
+        double turns = (double)(p0 + lo + first) * f;
+        turns -= rint(turns);
+        double s, c, ds, dc;
+        sincospi(2.0 * turns, &s, &c);
+        if (lastr - first > 1) sincospi(2.0 * (f - rint(f)), &ds, &dc);
+        c *= a.factor;
+        s *= a.factor;
+        for (int r = first; r < lastr; ++r) {
+          trig[((r * kQuads + e / 4) * turned + i / V) * 4 + e % 4] = (float)c;
+          trig[((r * kQuads + V / 4 + e / 4) * turned + i / V) * 4 + e % 4] = (float)s;
+          if (r + 1 < lastr) {
+            const double c2 = c * dc - s * ds;
+            s = s * dc + c * ds;
+            c = c2;
           }
         }
+      }
+      __syncthreads();
+    }
+    if (!active) continue;
+    for (int rb = lo + r0; rb < hi; rb += kBatch * step) {
+      uint4 u1[kBatch], u2[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) add_pair<T>(acc, u1[i], u2[i]);
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = rb + i * step;
+        if (r < hi) {
+          u1[i] = *reinterpret_cast<const uint4*>(in + r * in_step + c1);
+          u2[i] = *reinterpret_cast<const uint4*>(in + r * in_step + c2);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = rb + i * step;
+        if (r >= hi) break;
+        if (rotated) {
+          float4 cs[kQuads];
+#pragma unroll
+          for (int q = 0; q < kQuads; ++q)
+            cs[q] = reinterpret_cast<const float4*>(trig)[((r - lo) * kQuads + q) * turned + item];
+          turn<T, kMixed>(u1[i], u2[i], reinterpret_cast<const float*>(cs),
+                          reinterpret_cast<const float*>(cs + kQuads / 2));
+        }
+        if (sum) add_pair<T>(acc, u1[i], u2[i]);
+        const int64_t off = is_q ? r * a.o_stride[0] : at[r];
+        if (!is_q && off < 0) continue;  // its page is not there
+        *reinterpret_cast<uint4*>(out + off + c1) = u1[i];
+        *reinterpret_cast<uint4*>(out + off + c2) = u2[i];
       }
     }
-    if (active) {
-      for (int rb = r_lo + r0; rb < r_hi; rb += kBatch * step) {
-        uint4 u1[kBatch], u2[kBatch];
+  }
+  if (sum && h < heads) {
+    for (int o = items; o < 32; o <<= 1) {  // the other lanes' rows, into those with r0 = 0
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int r = rb + i * step;
-          if (r < r_hi) {
-            u1[i] = *reinterpret_cast<const uint4*>(in + r * in_step + c1);
-            u2[i] = *reinterpret_cast<const uint4*>(in + r * in_step + c2);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int r = rb + i * step;
-          if (r >= r_hi) break;
-          if (rotated) turn<T, kMixed>(u1[i], u2[i], cs + (r - r_lo) * half + item * V, sn + (r - r_lo) * half + item * V);
-          if (sum) add_pair<T>(acc, u1[i], u2[i]);
-          const int64_t off = is_q ? r * a.o_stride[0] : at[r];
-          if (!is_q && off < 0) continue;  // its page is not there
-          *reinterpret_cast<uint4*>(out + off + c1) = u1[i];
-          *reinterpret_cast<uint4*>(out + off + c2) = u2[i];
-        }
+      for (int i = 0; i < 2 * V; ++i) {
+        const float x = __shfl_down_sync(0xffffffffu, acc[i], o);
+        if (lane + o < 32) acc[i] += x;
       }
     }
-    if (sum) {
-      for (int o = items; o < 32; o <<= 1) {  // the other lanes' rows, into those with r0 = 0
+    if (r0 == 0) {
+      float* dst = is_q ? a.pooled_q + (((int64_t)b * a.Hq + hh) * a.NBq + qi) * a.D
+                        : a.pooled_k + (((int64_t)b * a.Hk + hh) * a.NBk + blk) * a.D;
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) {
-          const float x = __shfl_down_sync(0xffffffffu, acc[i], o);
-          if (lane + o < 32) acc[i] += x;
-        }
-      }
-      if (r0 == 0) {
-        float* dst = is_q ? a.pooled_q + (((int64_t)b * a.Hq + hh) * a.NBq + qi) * a.D
-                          : a.pooled_k + (((int64_t)b * a.Hk + hh) * a.NBk + blk) * a.D;
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-          *reinterpret_cast<float4*>(dst + c1 + i) =
-              make_float4(acc[i] / kRopeBlk, acc[i + 1] / kRopeBlk, acc[i + 2] / kRopeBlk, acc[i + 3] / kRopeBlk);
-          *reinterpret_cast<float4*>(dst + c2 + i) = make_float4(acc[V + i] / kRopeBlk, acc[V + i + 1] / kRopeBlk,
-                                                                 acc[V + i + 2] / kRopeBlk, acc[V + i + 3] / kRopeBlk);
-        }
+      for (int i = 0; i < V; i += 4) {
+        *reinterpret_cast<float4*>(dst + c1 + i) =
+            make_float4(acc[i] / kRopeBlk, acc[i + 1] / kRopeBlk, acc[i + 2] / kRopeBlk, acc[i + 3] / kRopeBlk);
+        *reinterpret_cast<float4*>(dst + c2 + i) = make_float4(acc[V + i] / kRopeBlk, acc[V + i + 1] / kRopeBlk,
+                                                               acc[V + i + 2] / kRopeBlk, acc[V + i + 3] / kRopeBlk);
       }
     }
   }
@@ -249,16 +260,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const tasft_r
 template <typename T, bool kMixed>
 int run(const tasft_rope_append_args& a, cudaStream_t st) {
   auto kern = rope_append_kernel<T, kMixed>;
-  const int smem = kRopeBlk * a.rot * (int)sizeof(float);  // cos and sin, rot / 2 each
+  const int smem = kRopeRows * a.rot * (int)sizeof(float);  // cos and sin, rot / 2 each
   static std::atomic<uint64_t> allowed{0};
-  if (smem > 48 * 1024 && !allow_smem(kern, kRopeBlk * 256 * (int)sizeof(float), allowed)) return TASFT_ERR_CUDA;
-  // shares of the heads: a warp's worth at least, more while CTAs are few
-  const int heads = a.Hq + 2 * a.Hk;
-  int64_t z = (4LL * sm_count() + (int64_t)a.B * a.NBq - 1) / ((int64_t)a.B * a.NBq);
-  const int most = (heads + 7) / 8;
-  if (z > most) z = most;
+  if (smem > 48 * 1024 && !allow_smem(kern, kRopeRows * 256 * (int)sizeof(float), allowed)) return TASFT_ERR_CUDA;
+  const int z = (a.Hq + 2 * a.Hk + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
   if (a.B > 65535) return TASFT_ERR_TOO_LARGE;
-  kern<<<dim3((unsigned)a.NBq, (unsigned)a.B, (unsigned)z), kRopeThreads, smem, st>>>(a);
+  kern<<<dim3((unsigned)z, (unsigned)a.NBq, (unsigned)a.B), kRopeThreads, smem, st>>>(a);
   count_launch();
   return launch_status();
 }
@@ -288,7 +295,7 @@ extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_s
       a.num_pages <= 0 || a.page_size <= 0)
     return TASFT_ERR_INVALID_ARG;
   if (!a.cu_seqlens || !a.kv_len || !a.block_table || !a.k_pages || !a.v_pages) return TASFT_ERR_INVALID_ARG;
-  if (a.NBq < (a.max_q + 126) / 64 || a.NBq > 1 << 20) return TASFT_ERR_INVALID_ARG;
+  if (a.NBq < (a.max_q + 126) / 64 || a.NBq > 65535) return TASFT_ERR_INVALID_ARG;
   if (a.pooled_k && a.NBk <= 0) return TASFT_ERR_INVALID_ARG;
   if (a.rot < 0 || a.rot > a.D || (a.rot > 0 && !a.inv_freq)) return TASFT_ERR_INVALID_ARG;
   if (a.k_stride[3] != 1 || a.v_stride[3] != 1) return TASFT_ERR_INVALID_ARG;
