@@ -5,7 +5,6 @@ fallback: if the shared object is missing or fails to load, every op raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 import struct
@@ -303,8 +302,6 @@ def strides3(t: torch.Tensor):
 
 
 def stream_ptr(device: torch.device) -> int:
-    if device.index is not None:
-        return torch._C._cuda_getCurrentRawStream(device.index)  # the handle without a Stream object (2 us)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -319,12 +316,13 @@ def packed(cls):
     return lambda *values: cls.from_buffer_copy(pack.pack(*values) + pad)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def on_device(t: torch.Tensor):
-    """Context in which t's device is the current one (launches go to the current device)."""
-    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+def launch(fn, args, gpu: int) -> int:
+    """Call a C entry point on device ``gpu``, on that device's current stream. (Launches go to the
+    current device; the raw handle spares the 2 us of a Stream object.)"""
+    if gpu == torch._C._cuda_getDevice():
+        return fn(args, torch._C._cuda_getCurrentRawStream(gpu))
+    with torch.cuda.device(gpu):
+        return fn(args, torch._C._cuda_getCurrentRawStream(gpu))
 
 
 def require_cuda(*ts: torch.Tensor) -> None:

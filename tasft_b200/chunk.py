@@ -198,19 +198,18 @@ def rope_append_paged(
         pooled_q = torch.empty(B, Hq, rows, D, dtype=torch.float32, device=dev)
         pq_ptr, pk_ptr = pooled_q.data_ptr(), pooled_k.data_ptr()
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != qs or out.dtype is not dtype or out.get_device() != gpu or out.stride(2) != 1:
         raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
     (q, qt), (k, kt), (v, vt) = _rows(q), _rows(k), _rows(v)
     freq = inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
-    with L.on_device(q):
-        args = _rope_args(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            qt[0], qt[1], kt[0], kt[1], vt[0], vt[1], out.stride(0), out.stride(1), *k_pages.stride(), *v_pages.stride(),
-            freq.data_ptr(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), pq_ptr, pk_ptr, attention_scaling,
-            B, T, Hq, Hk, D, 2 * freq.numel(), block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, rows,
-            nbk, interleaved, f64, err_ptr)
-        rc = L.lib().tasft_rope_append_paged(args, L.stream_ptr(dev))
+    args = _rope_args(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        qt[0], qt[1], kt[0], kt[1], vt[0], vt[1], out.stride(0), out.stride(1), *k_pages.stride(), *v_pages.stride(),
+        freq.data_ptr(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), pq_ptr, pk_ptr, attention_scaling,
+        B, T, Hq, Hk, D, 2 * freq.numel(), block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, rows,
+        nbk, interleaved, f64, err_ptr)
+    rc = L.launch(L.lib().tasft_rope_append_paged, args, gpu)
     if rc:
         L.check(rc, "tasft_rope_append_paged", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out, pooled_q
@@ -269,12 +268,11 @@ def select_blocks(
     dev = scores.device
     idx = torch.empty(B, num_kv_heads, nbq, width, dtype=torch.int32, device=dev)
     cnt = torch.empty(B, num_kv_heads, nbq, dtype=torch.int32, device=dev)
-    with L.on_device(scores):
-        args = _select_args(
-            scores.data_ptr(), st[0], st[1], st[2], cu.data_ptr(), kvl.data_ptr(), B, Hq, num_kv_heads, nbq, nbk, block,
-            min(top_k, nbk), min(first, nbk), min(local, nbk), tau is not None, 0.0 if tau is None else tau, width,
-            idx.data_ptr(), cnt.data_ptr(), err_ptr)
-        rc = L.lib().tasft_select_blocks(args, L.stream_ptr(dev))
+    args = _select_args(
+        scores.data_ptr(), st[0], st[1], st[2], cu.data_ptr(), kvl.data_ptr(), B, Hq, num_kv_heads, nbq, nbk, block,
+        min(top_k, nbk), min(first, nbk), min(local, nbk), tau is not None, 0.0 if tau is None else tau, width,
+        idx.data_ptr(), cnt.data_ptr(), err_ptr)
+    rc = L.launch(L.lib().tasft_select_blocks, args, gpu)
     if rc:
         L.check(rc, "tasft_select_blocks", shape=[B, Hq, num_kv_heads, nbq, nbk])
     return KeptBlocks(idx, cnt)
@@ -313,7 +311,6 @@ def bsa_chunk_paged(
     _check_pages(name, gpu, q, qs, k_pages, ks, v_pages)
     T, Hq, D = qs
     num_pages, page_size, Hk, _ = ks
-    dev = q.device
     B = kv_len.numel()
     kvl = _index(name, kv_len, gpu, B)
     cu = _index(name, cu_seqlens, gpu, B + 1)
@@ -340,7 +337,7 @@ def bsa_chunk_paged(
         idx_ptr, cnt_ptr = idx.data_ptr(), cnt.data_ptr()
         _, hm, rows, width = ls
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != qs or out.dtype is not q.dtype or out.get_device() != gpu or out.stride(2) != 1:
         raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
     st = q.stride()
@@ -348,17 +345,16 @@ def bsa_chunk_paged(
         q = q.contiguous()
         st = q.stride()
     lib = L.lib()
-    with L.on_device(q):
-        nbytes = lib.tasft_chunk_workspace_size(B, T, Hq, Hk, D, max_new, hm)
-        if nbytes < 0:
-            L.check(int(nbytes), "tasft_chunk_workspace_size", shape=[B, T, Hq, Hk, D])
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        args = _chunk_args(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), st[0], st[1], out.stride(0),
-            out.stride(1), *k_pages.stride(), *v_pages.stride(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), idx_ptr,
-            cnt_ptr, B, T, Hq, Hk, D, block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, hm, rows, width,
-            scale, ws.data_ptr(), nbytes, err_ptr)
-        rc = lib.tasft_bsa_chunk_paged_fwd(args, L.stream_ptr(dev))
+    nbytes = lib.tasft_chunk_workspace_size(B, T, Hq, Hk, D, max_new, hm)
+    if nbytes < 0:
+        L.check(int(nbytes), "tasft_chunk_workspace_size", shape=[B, T, Hq, Hk, D])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _chunk_args(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), st[0], st[1], out.stride(0), out.stride(1),
+        *k_pages.stride(), *v_pages.stride(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), idx_ptr, cnt_ptr, B, T, Hq,
+        Hk, D, block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, hm, rows, width, scale, ws.data_ptr(),
+        nbytes, err_ptr)
+    rc = L.launch(lib.tasft_bsa_chunk_paged_fwd, args, gpu)
     if rc:
         L.check(rc, "tasft_bsa_chunk_paged_fwd", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out

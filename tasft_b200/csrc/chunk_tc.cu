@@ -1178,8 +1178,11 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   int bound = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
   if (a.kept_idx && (int64_t)a.nb_w * 2 < bound) bound = a.nb_w * (sh.mode == 2 ? 2 : 1);
   sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
-  sh.may_cut = bound > kChunkMergeCost;  // else one launch
-  if (!a.workspace || a.workspace_bytes < ws_layout(sh, a.D, 2 * sm_count()).bytes) return TASFT_ERR_WORKSPACE;
+  // One launch where cutting tiles gains nothing: the gain is at most the last round's idle share
+  // of a tile as long as can be, for as many tiles as the tokens fill (the device decides the rest).
+  const int64_t G = 2 * sm_count(), tiles = ((int64_t)a.T / sh.tpt + a.B) * sh.units;
+  sh.may_cut = ((tiles + G - 1) / G * G - tiles) * bound > kChunkMergeCost * G;
+  if (!a.workspace || a.workspace_bytes < ws_layout(sh, a.D, (int)G).bytes) return TASFT_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   const bool f16 = a.dtype == TASFT_F16;
