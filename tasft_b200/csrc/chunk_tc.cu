@@ -26,12 +26,15 @@
 //         P read from TMEM where it overwrote S)
 //   2     lists: the next segment (at most kSeg entries) of block indices with their pages,
 //         double-buffered, ahead of the producer
-//   3     idle
+//   3     looks over the tiles of V that need it
 //   4-7   softmax, one thread per row; epilogue
 // Warps 0-3 hand registers to the second warpgroup (128 -> 88 and 168 a thread), each role at its
 // start: the compiler gives the code behind a common point the smaller count and spills.
-// Rows of V that no key stands for (past kv_len, or of a page that is not there) are zeroed in
-// shared memory before P.V, so what the cache holds there never meets a 0 of P.
+// A 0 of P must not meet what V holds behind the mask. Rows of V that no key stands for (past
+// kv_len, or of a page that is not there) are zeroed in shared memory before P.V. Where a block
+// holds keys that some row of the tile must not see, values that are not finite go to zero too,
+// and the rows that do see them take the infinity or NaN in the epilogue. Warp 3 does both while
+// the softmax of the block is under way.
 // Every mbarrier phase is indexed by a global counter and every wait is arranged so the waiter
 // is at most one phase behind; every wait is bounded (TASFT_DEVERR_TIMEOUT).
 #include "chunk.cuh"
@@ -113,6 +116,27 @@ struct ChunkWs {
   float* o;     // [2 CTAs, rows, D] sums not yet divided by l
 };
 
+// Which blocks of a tile warp 3 looks over.
+struct Look {
+  int lowest, slots;  // first position of the tile's tokens; slots in use
+  __device__ __forceinline__ Look(const Work& w, const ChunkShape& sh) {
+    lowest = w.pos[0];
+    slots = 1;
+    if (sh.mode == 2) {
+      lowest = min(w.valid[0] ? max(w.pos[0], w.ctx) : INT32_MAX, w.valid[1] ? max(w.pos[1], w.ctx) : INT32_MAX);
+      slots = (w.valid[0] ? 1 : 0) | (w.valid[1] ? 2 : 0);
+    }
+  }
+  // keys that some row of the tile must not see
+  __device__ __forceinline__ bool mixed(int entry, int kbase, int len) const {
+    return min(kbase + kChunkBlk, len) - 1 > lowest || ((entry >> (kKbBits + 4)) & slots) != slots;
+  }
+  // those, or rows of V without a key
+  __device__ __forceinline__ bool wanted(int entry, int kbase, int have, int all_pages, int len) const {
+    return have != all_pages || kbase + kChunkBlk > len || mixed(entry, kbase, len);
+  }
+};
+
 template <int D>
 struct Smem {
   static constexpr int kChunks = D / 64;                  // 64-element (128 B) swizzle atoms along D
@@ -127,13 +151,32 @@ struct Smem {
   static constexpr int kSumOff = kPageOff + 2 * kSeg * 16;        // [kChunkBuckets] int64, weight before
   static constexpr int kSeqOff = kSumOff + kChunkBuckets * 8;     // [kChunkBuckets] int4
   static constexpr int kBitmapOff = kSeqOff + kChunkBuckets * 16;  // [2][kSeg / 32]
-  static constexpr int kWorkOff = (kBitmapOff + 2 * (kSeg / 32) * 4 + 7) / 8 * 8;
+  static constexpr int kCodeOff = kBitmapOff + 2 * (kSeg / 32) * 4;  // [D / 16][128 rows]
+  static constexpr int kMarkOff = kCodeOff + (D / 16) * 128 * 4;  // softmax warps that still have to read them
+  static constexpr int kWorkOff = (kMarkOff + 8 + 7) / 8 * 8;
   static constexpr int kBarOff = (kWorkOff + 2 * (int)sizeof(Work) + 7) / 8 * 8;
-  static constexpr int kNumBars = 22;
+  static constexpr int kNumBars = 24;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kBytes = kMiscOff + 16;
   static constexpr int kAlloc = kBytes + 1024;  // slack for 1024-byte alignment
 };
+
+// Whether any of eight 16-bit values is not finite: exponents of all ones carry into the sign bits.
+template <bool kF16>
+__device__ __forceinline__ bool any_nonfinite(const uint4& u) {
+  constexpr uint32_t mask = kF16 ? 0x7c007c00u : 0x7f807f80u, one = kF16 ? 0x04000400u : 0x00800080u;
+  return ((((u.x & mask) + one) | ((u.y & mask) + one) | ((u.z & mask) + one) | ((u.w & mask) + one)) & 0x80008000u) != 0;
+}
+template <bool kF16>
+__device__ __forceinline__ bool nonfinite16(uint32_t v) {
+  constexpr uint32_t mask = kF16 ? 0x7c00u : 0x7f80u;
+  return (v & mask) == mask;
+}
+
+// 2-bit code of what values that are not finite make of a sum: 1 = +inf, 2 = -inf, 3 = NaN.
+__device__ __forceinline__ float nonfinite_of(uint32_t code, float v) {
+  return code == 0 ? v : code == 1 ? INFINITY : code == 2 ? -INFINITY : NAN;
+}
 
 struct PagedGeo {
   int nsub;       // pages of a block (page_size < 64)
@@ -164,9 +207,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* o_final = bars + 12;     // per tile: O complete
   uint64_t* o_free = bars + 13;      // per tile: epilogue has read O (one arrival per warp)
   uint64_t* list_full = bars + 14;   // [2] per segment
-  uint64_t* list_empty = bars + 16;  // [2] per segment (one arrival per softmax warp)
-  uint64_t* v_full = bars + 18;      // [2] per block
+  uint64_t* list_empty = bars + 16;  // [2] per segment (one arrival per softmax warp and one of warp 3)
+  uint64_t* v_full = bars + 18;      // [2] per block (by the copy, or by warp 3 where it looks over it)
   uint64_t* v_empty = bars + 20;     // [2] per block: P.V(g) has run
+  uint64_t* v_look = bars + 22;      // [2] per block whose V warp 3 looks over: it has landed
+  uint32_t* codes = reinterpret_cast<uint32_t*>(smem + L::kCodeOff);
+  volatile int32_t* mark = reinterpret_cast<volatile int32_t*>(smem + L::kMarkOff);
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -184,10 +230,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&p_ready[i], 4);
       mbar_init(&pv_done[i], 1);
       mbar_init(&list_full[i], 1);
-      mbar_init(&list_empty[i], 4);
+      mbar_init(&list_empty[i], 5);
     }
     mbar_init(o_final, 1);
     mbar_init(o_free, 4);
+    *mark = 0;
+    mbar_init(&v_look[0], 1);
+    mbar_init(&v_look[1], 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -594,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       tc::prefetch_tmap(&tmv);
       const int nsub = max(1, kChunkBlk / a.page_size), sub_rows = min(kChunkBlk, a.page_size);
       const uint32_t q_bytes = sh.mode == 2 ? 0 : (uint32_t)(L::kChunks * sh.hpt * sh.tpt * 128);
-      int gk = 0, tile = 0;
+      const int all_pages = (1 << nsub) - 1;
+      int gk = 0, tile = 0, looks = 0;
       bool ok = true;
       for (int u = 0; ok; ++u) {
         const int lb = u & 1;
@@ -621,19 +671,21 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         const int32_t* list = lists + lb * kSeg;
         const int32_t* pgs = reinterpret_cast<const int32_t*>(pages + lb * kSeg);
+        const Look look(w, sh);
         // one entry's K or V: the share of each page it has, into the stage's rows
         auto load = [&](int gi, int j, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off) -> bool {
           const int st = gi & 1;
           if (gi >= 2 && !mbar_wait(&empty[st], ((gi >> 1) - 1) & 1)) return false;
-          const int e = list[j], have = (e >> kKbBits) & 15;
+          const int e = list[j], have = (e >> kKbBits) & 15, kbase = (e & kKbMask) * kChunkBlk;
           const int in_page = a.page_size > kChunkBlk ? ((e & kKbMask) & 1) * kChunkBlk : 0;
           uint8_t* dst = smem + L::kStageOff + off + st * L::kKVTileBytes;
-          mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * L::kChunks * sub_rows * 128));
+          uint64_t* bar = &full[st];
+          if (full == v_full && look.wanted(e, kbase, have, all_pages, w.len)) bar = &v_look[looks++ & 1];
+          mbar_arrive_expect_tx(bar, (uint32_t)(__popc(have) * L::kChunks * sub_rows * 128));
           for (int x = 0; x < nsub; ++x) {
             if (!((have >> x) & 1)) continue;
             for (int c = 0; c < L::kChunks; ++c)
-              tc::tma_load_4d(dst + c * 64 * 128 + x * sub_rows * 128, map, c * 64, w.hk, in_page, pgs[4 * j + x],
-                              &full[st]);
+              tc::tma_load_4d(dst + c * 64 * 128 + x * sub_rows * 128, map, c * 64, w.hk, in_page, pgs[4 * j + x], bar);
           }
           return true;
         };
@@ -843,18 +895,6 @@ __global__ void __launch_bounds__(kThreads, 2)
           tc::tmem_st32(tS0 + (gi & 1) * 64 + lane_off, pk);
           tc::tmem_wait_st();
         }
-        if (have != all_pages || kbase + kChunkBlk > len) {
-          // rows of V that stand for no key are zeroed (V(gi + 2) cannot land before this
-          // block's P.V, which waits for these threads: the wait below is at most a phase behind)
-          if (!warp_wait(&v_full[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
-          uint8_t* vt = smem + L::kStageOff + L::kVOff + (gi & 1) * L::kKVTileBytes;
-          for (int i = r; i < 64 * L::kChunks * 8; i += 128) {  // 16-byte pieces
-            const int vr = (i >> 3) & 63;
-            if (kbase + vr >= len || !((have >> (vr / sub_rows)) & 1))
-              reinterpret_cast<uint4*>(vt)[i] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
         warp_arrive(&p_ready[gi & 1], lane);
         started = true;
       }
@@ -863,6 +903,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (last) {
         if (!warp_wait(o_final, tile & 1)) { ok = false; break; }
         tc::tc_fence_after();
+        const bool marked = *mark != 0;  // this tile's: warp 3 waits for them to be read
+        const uint32_t* code = codes + r;
         if (!any_live) {
         } else if (w->part < 0) {
           T* orow = reinterpret_cast<T*>(a.out) + (int64_t)(w->row[slot] + tok) * a.o_stride[0] +
@@ -880,8 +922,12 @@ __global__ void __launch_bounds__(kThreads, 2)
               uint32_t pk[16];
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
-                const float v0 = __uint_as_float(o[2 * c]) * inv;
-                const float v1 = __uint_as_float(o[2 * c + 1]) * inv;
+                float v0 = __uint_as_float(o[2 * c]) * inv, v1 = __uint_as_float(o[2 * c + 1]) * inv;
+                if (marked) {
+                  const uint32_t cd = code[((c0 + 2 * c) >> 4) * 128] >> (((c0 + 2 * c) & 15) * 2);
+                  v0 = nonfinite_of(cd & 3, v0);
+                  v1 = nonfinite_of((cd >> 2) & 3, v1);
+                }
                 pk[c] = kF16 ? tc::pack_f16x2(v0, v1) : tc::pack_bf16x2(v0, v1);
               }
               uint4* dst = reinterpret_cast<uint4*>(orow + c0);
@@ -896,6 +942,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int c0 = 0; c0 < D; c0 += 32) {
               uint32_t o[32];
               tc::tmem_ld32_sync(tO + c0 + lane_off, o);
+              if (marked) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  o[c] = __float_as_uint(nonfinite_of((code[((c0 + c) >> 4) * 128] >> (((c0 + c) & 15) * 2)) & 3, __uint_as_float(o[c])));
+              }
               if (live) {
                 float4* dst = reinterpret_cast<float4*>(ws.o + prow * D + c0);
 #pragma unroll
@@ -906,13 +957,102 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
+        if (marked) {
+          __syncwarp();
+          if (lane == 0) atomicSub(const_cast<int32_t*>(mark), 1);
+        }
         warp_arrive(o_free, lane);
       }
       warp_arrive(&list_empty[lb], lane);
     }
     if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 12));
   } else {
+    // ================= looking over V (warp 3) =================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int sub_rows = min(kChunkBlk, a.page_size);
+    const int all_pages = (1 << max(1, kChunkBlk / a.page_size)) - 1;
+    int g = 0, tile = -1, looks = 0, open = -1;  // open: the tile whose codes are being collected
+    bool ok = true;
+    for (int u = 0; ok; ++u) {
+      const int lb = u & 1;
+      if (!warp_wait(&list_full[lb], (u >> 1) & 1)) { ok = false; break; }
+      const Work* w = &works[lb];
+      const int n = w->n, len = w->len;
+      if (n < 0) break;
+      if (w->first) ++tile;
+      const Look look(*w, sh);
+      for (int j = 0; j < n; ++j) {
+        const int gi = g + j, entry = lists[lb * kSeg + j];
+        const int kbase = (entry & kKbMask) * kChunkBlk, have = (entry >> kKbBits) & 15;
+        if (!look.wanted(entry, kbase, have, all_pages, len)) continue;
+        if (!warp_wait(&v_look[looks & 1], (looks >> 1) & 1)) { ok = false; break; }
+        ++looks;
+        const bool mixed = look.mixed(entry, kbase, len);
+        uint4* vt = reinterpret_cast<uint4*>(smem + L::kStageOff + L::kVOff + (gi & 1) * L::kKVTileBytes);
+        uint64_t keys = 0;  // rows of the tile that stand for a key
+        for (int x = 0; x * sub_rows < kChunkBlk; ++x)
+          if ((have >> x) & 1) keys |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
+        if (kbase + kChunkBlk > len) keys &= (1ull << (len - kbase)) - 1;
+        bool bad = false;
+#pragma unroll 4
+        for (int i = lane; i < 64 * L::kChunks * 8; i += 32) {  // 16-byte pieces
+          if (!((keys >> ((i >> 3) & 63)) & 1)) vt[i] = make_uint4(0, 0, 0, 0);
+          else if (mixed) bad |= any_nonfinite<kF16>(vt[i]);
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+          if (open != tile) {  // once an earlier tile's codes have been read
+            const uint64_t t0 = globaltimer_ns();
+            while (*mark != 0 && globaltimer_ns() - t0 < kWaitLimitNs) {}
+            if (*mark != 0) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            for (int i = lane; i < (D / 16) * 128; i += 32) codes[i] = 0;
+            __syncwarp();
+            if (lane == 0) *mark = 4;
+            open = tile;
+          }
+          for (int q = 0; q < 4; ++q) {
+            const int r = q * 32 + lane, slot = sh.mode == 2 ? r >> 6 : 0;
+            const int tok = sh.mode == 2 ? r & 63 : r / sh.hpt;
+            const bool use = sh.mode == 2 ? ((entry >> (kKbBits + 4 + slot)) & 1) != 0 : tok < w->valid[0];
+            const int lim = max(0, min(w->pos[slot] + tok - kbase + 1, kChunkBlk));
+            const uint64_t seen = !use || lim == 0 ? 0 : keys & (lim == 64 ? ~0ull : (1ull << lim) - 1);
+            for (int c = 0; c < 64; ++c) {
+              if (!((seen >> c) & 1)) continue;
+              for (int i = 0; i < D / 8; ++i) {
+                const uint4 v = vt[(i >> 3) * 512 + c * 8 + (i & 7)];
+                if (!any_nonfinite<kF16>(v)) continue;
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t v2 = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+                  const uint32_t x = (v2 >> ((e & 1) * 16)) & 0xffffu;
+                  if (!nonfinite16<kF16>(x)) continue;
+                  const int d = (i >> 3) * 64 + (((i & 7) ^ (c & 7)) << 3) + e;  // 128B swizzle
+                  const uint32_t kind = (x & (kF16 ? 0x3ffu : 0x7fu)) ? 3u : (x & 0x8000u) ? 2u : 1u;
+                  codes[(d >> 4) * 128 + r] |= kind << ((d & 15) * 2);
+                }
+              }
+            }
+          }
+          __syncwarp();  // every row has its codes: the values go
+          for (int i = lane; i < 64 * L::kChunks * 8; i += 32) {
+            uint4 v = vt[i];
+            if (!any_nonfinite<kF16>(v)) continue;
+            uint32_t* x = &v.x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (nonfinite16<kF16>((x[e >> 1] >> ((e & 1) * 16)) & 0xffffu)) x[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+            vt[i] = v;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[gi & 1]);
+      }
+      g += n;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_empty[lb]);
+    }
+    if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 13));
   }
   // ---------------- teardown ----------------
   __syncwarp();

@@ -205,6 +205,60 @@ def test_sequences_that_do_not_fit_are_left_out():
     assert int(err.item()) & 1
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("lists", [None, "kv", "q"])
+@pytest.mark.parametrize("n", [100, 2])
+def test_values_not_finite_reach_only_rows_that_see_them(dtype, D, lists, n):
+    """Infinities and NaN of K and V at some positions: rows before them, and rows whose lists skip
+    their block, are as if they were not there; rows that see them give what the sums give."""
+    new, ctx, Hq, Hk = [n], [230], 4, 2
+    q, kp, vp, table, cu, kv_len, g = case(new, ctx, Hq, Hk, D, 16, dtype, 16)
+    total = n + 230
+    kept = None
+    if lists is not None:
+        kept = T.KeptBlocks(*R.random_lists(new, ctx, Hk if lists == "kv" else Hq, 6, DEV, g, 0.6))
+        kept = T.KeptBlocks(kept.idx, kept.cnt)
+    bad = {total - 1: (3, math.inf), total - 2: (3, -math.inf), 231: (7, math.nan), 70: (D - 1, -math.inf)}
+    vz = vp.clone()
+    at = lambda t: (int(table[0, t // 16]), t % 16)  # noqa: E731
+    for t, (d, x) in bad.items():
+        vp[at(t)[0], at(t)[1], :, d] = x
+        vz[at(t)[0], at(t)[1], :, d] = 0.0
+    o, a = R.attend(q, kp, vz, table, new, ctx, None if kept is None else (kept.idx, kept.cnt))
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, n, kept, err=err)
+    assert int(err.item()) == 0
+    bound = R.attend_bound(o, a, dtype, total)
+    want = o.clone()
+    pos = 230 + torch.arange(n, device=DEV)
+    for h in range(Hq):
+        for t, (d, x) in bad.items():
+            see = pos >= t
+            if kept is not None:
+                lists_h = kept.idx[0, h if lists == "q" else h // 2].long()
+                see = see & (lists_h == t // 64).any(1)[pos // 64 - 230 // 64]
+            want[see, h, d] += x
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), finite)
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out.double()[~finite & ~torch.isnan(want)], want[~finite & ~torch.isnan(want)])
+    assert ((out.double() - o).abs()[finite] <= bound[finite]).all()
+    # keys that are not finite, behind every row's mask but the last one's
+    kp[at(total - 1)[0], at(total - 1)[1]] = math.nan
+    again = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, n, kept)
+    assert torch.equal(again[:-1].nan_to_num(5), out[:-1].nan_to_num(5))
+
+
+def test_a_query_that_is_nan_gives_nan():
+    q, kp, vp, table, cu, kv_len, g = case([40], [100], 4, 2, 128, 16, torch.bfloat16, 17)
+    good = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, 40)
+    q[7, 2] = math.nan
+    out = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, 40)
+    assert torch.isnan(out[7, 2]).all()
+    out[7, 2] = good[7, 2]
+    assert torch.equal(out, good)
+
+
 def test_graph_replay_follows_its_inputs():
     new, ctx = [33, 1, 1], [500, 900, 40]
     q, kp, vp, table, cu, kv_len, g = case(new, ctx, 8, 2, 128, 16, torch.bfloat16, 15)
