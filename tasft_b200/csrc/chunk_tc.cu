@@ -20,7 +20,7 @@
 // the same cuts from cu_seqlens and kv_len, so the host needs neither. A CTA takes its length from
 // the back: the piece at its end starts at block 0 and the one at its start ends at the last, so
 // CTAs that share K and V run over them side by side and find them in L2. Warps:
-//   0     producer: Q of the tile, then K and V of every entry through separate 2-stage rings
+//   0     producer: Q of the tile, then K and V of every entry through separate rings
 //         (TMA from the pages, 128B swizzle)
 //   1     MMA issuer: S = Q K^T (SS, M128 N64) into a double-buffered TMEM tile, O += P V (TS:
 //         P read from TMEM where it overwrote S)
@@ -142,11 +142,12 @@ struct Smem {
   static constexpr int kChunks = D / 64;                  // 64-element (128 B) swizzle atoms along D
   static constexpr int kQBytes = kChunks * 128 * 128;
   static constexpr int kKVTileBytes = kChunks * 64 * 128;
+  static constexpr int kRing = D == 64 ? 4 : 2;            // stages of K and of V (64 KB together)
   static constexpr int kKOff = 0;
-  static constexpr int kVOff = 2 * kKVTileBytes;
+  static constexpr int kVOff = kRing * kKVTileBytes;
   static constexpr int kQOff = 0;
   static constexpr int kStageOff = kQOff + kQBytes;
-  static constexpr int kListOff = kStageOff + 4 * kKVTileBytes;  // [2][kSeg] entries
+  static constexpr int kListOff = kStageOff + 2 * kRing * kKVTileBytes;  // [2][kSeg] entries
   static constexpr int kPageOff = kListOff + 2 * kSeg * 4;       // [2][kSeg][4] pages
   static constexpr int kSumOff = kPageOff + 2 * kSeg * 16;        // [kChunkBuckets] int64, weight before
   static constexpr int kSeqOff = kSumOff + kChunkBuckets * 8;     // [kChunkBuckets] int4
@@ -155,7 +156,7 @@ struct Smem {
   static constexpr int kMarkOff = kCodeOff + (D / 16) * 128 * 4;  // softmax warps that still have to read them
   static constexpr int kWorkOff = (kMarkOff + 8 + 7) / 8 * 8;
   static constexpr int kBarOff = (kWorkOff + 2 * (int)sizeof(Work) + 7) / 8 * 8;
-  static constexpr int kNumBars = 24;
+  static constexpr int kNumBars = 14 + 5 * kRing;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kBytes = kMiscOff + 16;
   static constexpr int kAlloc = kBytes + 1024;  // slack for 1024-byte alignment
@@ -199,18 +200,18 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* q_full = bars + 0;       // per tile: Q landed
   uint64_t* q_empty = bars + 1;      // per tile: every S of the tile has run (Q reusable)
-  uint64_t* k_full = bars + 2;       // [2] per block
-  uint64_t* k_empty = bars + 4;      // [2] per block: S(g) has run
-  uint64_t* s_full = bars + 6;       // [2] per block
-  uint64_t* p_ready = bars + 8;      // [2] per block (one arrival per softmax warp)
-  uint64_t* pv_done = bars + 10;     // [2] per block: P.V(g) has run
-  uint64_t* o_final = bars + 12;     // per tile: O complete
-  uint64_t* o_free = bars + 13;      // per tile: epilogue has read O (one arrival per warp)
-  uint64_t* list_full = bars + 14;   // [2] per segment
-  uint64_t* list_empty = bars + 16;  // [2] per segment (one arrival per softmax warp and one of warp 3)
-  uint64_t* v_full = bars + 18;      // [2] per block (by the copy, or by warp 3 where it looks over it)
-  uint64_t* v_empty = bars + 20;     // [2] per block: P.V(g) has run
-  uint64_t* v_look = bars + 22;      // [2] per block whose V warp 3 looks over: it has landed
+  uint64_t* o_final = bars + 2;      // per tile: O complete
+  uint64_t* o_free = bars + 3;       // per tile: epilogue has read O (one arrival per warp)
+  uint64_t* s_full = bars + 4;       // [2] per block
+  uint64_t* p_ready = bars + 6;      // [2] per block (one arrival per softmax warp)
+  uint64_t* pv_done = bars + 8;      // [2] per block: P.V(g) has run
+  uint64_t* list_full = bars + 10;   // [2] per segment
+  uint64_t* list_empty = bars + 12;  // [2] per segment (one arrival per softmax warp and one of warp 3)
+  uint64_t* k_full = bars + 14;              // [kRing] per block
+  uint64_t* k_empty = k_full + L::kRing;     // [kRing] per block: S(g) has run
+  uint64_t* v_full = k_empty + L::kRing;     // [kRing] per block (by the copy, or by warp 3 where it looks over it)
+  uint64_t* v_empty = v_full + L::kRing;     // [kRing] per block: P.V(g) has run
+  uint64_t* v_look = v_empty + L::kRing;     // [kRing] per block whose V warp 3 looks over: it has landed
   uint32_t* codes = reinterpret_cast<uint32_t*>(smem + L::kCodeOff);
   volatile int32_t* mark = reinterpret_cast<volatile int32_t*>(smem + L::kMarkOff);
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
@@ -221,11 +222,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 0 && lane == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < L::kRing; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_look[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);
       mbar_init(&pv_done[i], 1);
@@ -235,8 +239,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(o_final, 1);
     mbar_init(o_free, 4);
     *mark = 0;
-    mbar_init(&v_look[0], 1);
-    mbar_init(&v_look[1], 1);
+
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -674,13 +677,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         const Look look(w, sh);
         // one entry's K or V: the share of each page it has, into the stage's rows
         auto load = [&](int gi, int j, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off) -> bool {
-          const int st = gi & 1;
-          if (gi >= 2 && !mbar_wait(&empty[st], ((gi >> 1) - 1) & 1)) return false;
+          const int st = gi % L::kRing;
+          if (gi >= L::kRing && !mbar_wait(&empty[st], (gi / L::kRing - 1) & 1)) return false;
           const int e = list[j], have = (e >> kKbBits) & 15, kbase = (e & kKbMask) * kChunkBlk;
           const int in_page = a.page_size > kChunkBlk ? ((e & kKbMask) & 1) * kChunkBlk : 0;
           uint8_t* dst = smem + L::kStageOff + off + st * L::kKVTileBytes;
           uint64_t* bar = &full[st];
-          if (full == v_full && look.wanted(e, kbase, have, all_pages, w.len)) bar = &v_look[looks++ & 1];
+          if (full == v_full && look.wanted(e, kbase, have, all_pages, w.len)) bar = &v_look[looks++ % L::kRing];
           mbar_arrive_expect_tx(bar, (uint32_t)(__popc(have) * L::kChunks * sub_rows * 128));
           for (int x = 0; x < nsub; ++x) {
             if (!((have >> x) & 1)) continue;
@@ -699,9 +702,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 10));
       // do not leave while copies into shared memory are in flight
       if (tile > 0) mbar_wait(q_full, (tile - 1) & 1);
-      for (int i = max(0, gk - 2); ok && i < gk; ++i) {
-        mbar_wait(&k_full[i & 1], (i >> 1) & 1);
-        mbar_wait(&v_full[i & 1], (i >> 1) & 1);
+      for (int i = max(0, gk - L::kRing); ok && i < gk; ++i) {
+        mbar_wait(&k_full[i % L::kRing], (i / L::kRing) & 1);
+        mbar_wait(&v_full[i % L::kRing], (i / L::kRing) & 1);
       }
     }
   } else if (warp == 1) {
@@ -715,12 +718,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       int g = 0, tile = -1;
       bool ok = true, started = false;
       auto issue_s = [&](int gi) -> bool {
-        const int st = gi & 1;
-        if (!mbar_wait(&k_full[st], (gi >> 1) & 1)) return false;
+        const int st = gi & 1, kst = gi % L::kRing;
+        if (!mbar_wait(&k_full[kst], (gi / L::kRing) & 1)) return false;
         // S(gi) overwrites P(gi - 2) in TMEM: P.V(gi - 2) was issued earlier by this thread, and
         // the MMAs of one thread run through the tensor pipe in issue order
         tc::tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + L::kStageOff + L::kKOff + st * L::kKVTileBytes);
+        const uint32_t k_addr = smem_u32(smem + L::kStageOff + L::kKOff + kst * L::kKVTileBytes);
         const uint32_t dst = tS0 + st * 64;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -729,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           tc::mma_ss(dst, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
         }
         tc::mma_commit(&s_full[st]);
-        tc::mma_commit(&k_empty[st]);
+        tc::mma_commit(&k_empty[kst]);
         return true;
       };
       for (int u = 0; ok; ++u) {
@@ -755,9 +758,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!mbar_wait(&p_ready[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
           // O is reused: the previous tile's epilogue must have read it
           if (!started && tile >= 1 && !mbar_wait(o_free, (tile - 1) & 1)) { ok = false; break; }
-          if (!mbar_wait(&v_full[gi & 1], (gi >> 1) & 1)) { ok = false; break; }
+          const int vst = gi % L::kRing;
+          if (!mbar_wait(&v_full[vst], (gi / L::kRing) & 1)) { ok = false; break; }
           tc::tc_fence_after();
-          const uint32_t v_addr = smem_u32(smem + L::kStageOff + L::kVOff + (gi & 1) * L::kKVTileBytes);
+          const uint32_t v_addr = smem_u32(smem + L::kStageOff + L::kVOff + vst * L::kKVTileBytes);
           const uint32_t p_tmem = tS0 + (gi & 1) * 64;
 #pragma unroll
           for (int kk = 0; kk < kChunkBlk / 16; ++kk) {
@@ -765,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             tc::mma_ts(tO, p_tmem + kk * 8, bd, idesc_o, (started || kk > 0) ? 1u : 0u);
           }
           started = true;
-          tc::mma_commit(&v_empty[gi & 1]);
+          tc::mma_commit(&v_empty[vst]);
           tc::mma_commit(&pv_done[gi & 1]);
         }
         if (!ok) break;
@@ -985,17 +989,25 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int gi = g + j, entry = lists[lb * kSeg + j];
         const int kbase = (entry & kKbMask) * kChunkBlk, have = (entry >> kKbBits) & 15;
         if (!look.wanted(entry, kbase, have, all_pages, len)) continue;
-        if (!warp_wait(&v_look[looks & 1], (looks >> 1) & 1)) { ok = false; break; }
+        if (!warp_wait(&v_look[looks % L::kRing], (looks / L::kRing) & 1)) { ok = false; break; }
         ++looks;
         const bool mixed = look.mixed(entry, kbase, len);
-        uint4* vt = reinterpret_cast<uint4*>(smem + L::kStageOff + L::kVOff + (gi & 1) * L::kKVTileBytes);
+        uint4* vt = reinterpret_cast<uint4*>(smem + L::kStageOff + L::kVOff + (gi % L::kRing) * L::kKVTileBytes);
         uint64_t keys = 0;  // rows of the tile that stand for a key
         for (int x = 0; x * sub_rows < kChunkBlk; ++x)
           if ((have >> x) & 1) keys |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
         if (kbase + kChunkBlk > len) keys &= (1ull << (len - kbase)) - 1;
         bool bad = false;
-#pragma unroll 4
-        for (int i = lane; i < 64 * L::kChunks * 8; i += 32) {  // 16-byte pieces
+        if (keys == ~0ull) {  // (so it is looked over for its values; eight loads in flight)
+#pragma unroll
+          for (int i0 = 0; i0 < 64 * L::kChunks * 8; i0 += 256) {
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = vt[i0 + i * 32 + lane];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bad |= any_nonfinite<kF16>(v[i]);
+          }
+        } else for (int i = lane; i < 64 * L::kChunks * 8; i += 32) {  // 16-byte pieces
           if (!((keys >> ((i >> 3) & 63)) & 1)) vt[i] = make_uint4(0, 0, 0, 0);
           else if (mixed) bad |= any_nonfinite<kF16>(vt[i]);
         }
@@ -1046,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[gi & 1]);
+        if (lane == 0) mbar_arrive(&v_full[gi % L::kRing]);
       }
       g += n;
       __syncwarp();
