@@ -153,7 +153,7 @@ struct Smem {
   static constexpr int kSeqOff = kSumOff + kChunkBuckets * 8;     // [kChunkBuckets] int4
   static constexpr int kBitmapOff = kSeqOff + kChunkBuckets * 16;  // [2][kSeg / 32]
   static constexpr int kCodeOff = kBitmapOff + 2 * (kSeg / 32) * 4;  // [D / 16][128 rows]
-  static constexpr int kMarkOff = kCodeOff + (D / 16) * 128 * 4;  // softmax warps that still have to read them
+  static constexpr int kMarkOff = kCodeOff + (D / 16) * 128 * 4;  // tile << 3 | softmax warps that still have to read them
   static constexpr int kWorkOff = (kMarkOff + 8 + 7) / 8 * 8;
   static constexpr int kBarOff = (kWorkOff + 2 * (int)sizeof(Work) + 7) / 8 * 8;
   static constexpr int kNumBars = 14 + 5 * kRing;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* p_ready = bars + 6;      // [2] per block (one arrival per softmax warp)
   uint64_t* pv_done = bars + 8;      // [2] per block: P.V(g) has run
   uint64_t* list_full = bars + 10;   // [2] per segment
-  uint64_t* list_empty = bars + 12;  // [2] per segment (one arrival per softmax warp and one of warp 3)
+  uint64_t* list_empty = bars + 12;  // [2] per segment (arrivals: four softmax warps, warps 0 and 3)
   uint64_t* k_full = bars + 14;              // [kRing] per block
   uint64_t* k_empty = k_full + L::kRing;     // [kRing] per block: S(g) has run
   uint64_t* v_full = k_empty + L::kRing;     // [kRing] per block (by the copy, or by warp 3 where it looks over it)
@@ -234,12 +234,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&p_ready[i], 4);
       mbar_init(&pv_done[i], 1);
       mbar_init(&list_full[i], 1);
-      mbar_init(&list_empty[i], 5);
+      mbar_init(&list_empty[i], 6);
     }
     mbar_init(o_final, 1);
     mbar_init(o_free, 4);
     *mark = 0;
-
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -404,7 +403,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int64_t edge = 2 * kChunkBlk, back = from.rho - step;
       recorded = back >= edge && blockIdx.x > 0;
     }
-    if (recorded && lane == 0) ws.cut[blockIdx.x].pieces = 0;
+    // (a CTA that gives up leaves no record: the merge then does nothing for it)
+    if (lane == 0) ws.cut[blockIdx.x].pieces = 0;
+    __syncwarp();
 
     int u = 0;  // segment counter
     bool ok = true;
@@ -623,7 +624,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         __syncwarp();
         const bool last = at >= hi;
-        if (sh.mode == 2 && n == 0 && !last) continue;  // an empty window: the next one
+        // nothing kept here: on to the next (the MMA issuer could fall two empty segments behind)
+        if (n == 0 && !last) continue;
         if (lane == 0) {
           w.n = n;
           w.first = first;
@@ -647,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int nsub = max(1, kChunkBlk / a.page_size), sub_rows = min(kChunkBlk, a.page_size);
       const uint32_t q_bytes = sh.mode == 2 ? 0 : (uint32_t)(L::kChunks * sh.hpt * sh.tpt * 128);
       const int all_pages = (1 << nsub) - 1;
-      int gk = 0, tile = 0, looks = 0;
+      int gk = 0, gv = 0, tile = 0, looks = 0;  // K and V tiles asked for, tiles, V tiles for warp 3
       bool ok = true;
       for (int u = 0; ok; ++u) {
         const int lb = u & 1;
@@ -694,18 +696,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         };
         // K(j) then V(j-1): the order the MMA warp consumes them
         for (int j = 0; ok && j <= n && n > 0; ++j) {
-          if (j < n && !load(gk + j, j, &tmk, k_full, k_empty, L::kKOff)) ok = false;
-          if (ok && j >= 1 && !load(gk + j - 1, j - 1, &tmv, v_full, v_empty, L::kVOff)) ok = false;
+          if (j < n) {
+            ok = load(gk, j, &tmk, k_full, k_empty, L::kKOff);
+            if (ok) ++gk;
+          }
+          if (ok && j >= 1) {
+            ok = load(gv, j - 1, &tmv, v_full, v_empty, L::kVOff);
+            if (ok) ++gv;
+          }
         }
-        gk += n;
+        // the softmax warps may be through with the segment while its last V is not on its way yet
+        if (ok) mbar_arrive(&list_empty[lb]);
       }
       if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 10));
-      // do not leave while copies into shared memory are in flight
+      // do not leave while copies into shared memory are in flight, after a timeout either
       if (tile > 0) mbar_wait(q_full, (tile - 1) & 1);
-      for (int i = max(0, gk - L::kRing); ok && i < gk; ++i) {
-        mbar_wait(&k_full[i % L::kRing], (i / L::kRing) & 1);
-        mbar_wait(&v_full[i % L::kRing], (i / L::kRing) & 1);
-      }
+      for (int i = max(0, gk - L::kRing); i < gk; ++i) mbar_wait(&k_full[i % L::kRing], (i / L::kRing) & 1);
+      for (int i = max(0, looks - L::kRing); i < looks; ++i) mbar_wait(&v_look[i % L::kRing], (i / L::kRing) & 1);
+      for (int i = max(0, gv - L::kRing); i < gv; ++i) mbar_wait(&v_full[i % L::kRing], (i / L::kRing) & 1);
     }
   } else if (warp == 1) {
     // ================= MMA issuer =================
@@ -907,7 +915,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (last) {
         if (!warp_wait(o_final, tile & 1)) { ok = false; break; }
         tc::tc_fence_after();
-        const bool marked = *mark != 0;  // this tile's: warp 3 waits for them to be read
+        const int tag = *mark;  // warp 3 may be at the next tile already
+        const bool marked = (tag >> 3) == tile && (tag & 7) != 0;
         const uint32_t* code = codes + r;
         if (!any_live) {
         } else if (w->part < 0) {
@@ -1014,13 +1023,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (__any_sync(0xffffffffu, bad)) {
           if (open != tile) {  // once an earlier tile's codes have been read
             const uint64_t t0 = globaltimer_ns();
-            while (*mark != 0 && globaltimer_ns() - t0 < kWaitLimitNs) {}
-            if (*mark != 0) ok = false;
+            while ((*mark & 7) != 0 && globaltimer_ns() - t0 < kWaitLimitNs) {}
+            if ((*mark & 7) != 0) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             for (int i = lane; i < (D / 16) * 128; i += 32) codes[i] = 0;
             __syncwarp();
-            if (lane == 0) *mark = 4;
+            if (lane == 0) *mark = (tile << 3) | 4;
             open = tile;
           }
           for (int q = 0; q < 4; ++q) {
@@ -1090,7 +1099,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const tasft_
   const int c = blockIdx.x;
   const Work w = ws.cut[c];
   const int ns = w.pieces;
-  if (ns == 0) return;
+  if (ns < 2 || c + ns - 2 >= (int)gridDim.x) return;
   const int warp = threadIdx.x >> 5;
   // where a row of the tile goes, or null
   auto target = [&](int r) -> T* {
