@@ -209,16 +209,16 @@ class GateBwdArgs(C.Structure):
     ]
 
 
-# name -> (argtypes, restype); every symbol declared in include/tasft_b200.h
+# name -> (argtypes, restype), vp for an argument block that may come as packed bytes; every symbol declared in include/tasft_b200.h
 SIGNATURES = {
     "tasft_gate_workspace_size": ([C.c_int32] * 8, C.c_int64),
     "tasft_gate_mask_build": ([C.POINTER(GateArgs), vp], C.c_int),
     "tasft_mask_from_scores": ([C.POINTER(ThresholdArgs), vp], C.c_int),
     "tasft_qkv_rope_pool": ([C.POINTER(QkvArgs), vp], C.c_int),
-    "tasft_rope_append_paged": ([C.POINTER(RopeAppendArgs), vp], C.c_int),
-    "tasft_select_blocks": ([C.POINTER(SelectArgs), vp], C.c_int),
+    "tasft_rope_append_paged": ([vp, vp], C.c_int),
+    "tasft_select_blocks": ([vp, vp], C.c_int),
     "tasft_chunk_workspace_size": ([C.c_int32] * 7, C.c_int64),
-    "tasft_bsa_chunk_paged_fwd": ([C.POINTER(ChunkArgs), vp], C.c_int),
+    "tasft_bsa_chunk_paged_fwd": ([vp, vp], C.c_int),
     "tasft_mask_to_kept": ([C.POINTER(MaskArgs), vp], C.c_int),
     "tasft_calibrate_tau": ([C.POINTER(CalibArgs), vp], C.c_int),
     "tasft_bsa_prefill_fwd": ([C.POINTER(PrefillArgs), vp], C.c_int),
@@ -306,14 +306,13 @@ def stream_ptr(device: torch.device) -> int:
 
 
 def packed(cls):
-    """A constructor of ``cls`` from its fields' plain values in order, arrays flattened and null
-    pointers as 0: one struct.pack, a third of the time that ctypes takes field by field."""
+    """The bytes of a ``cls`` from its fields' plain values in order, arrays flattened and null
+    pointers as 0: one struct.pack, a quarter of the time that ctypes takes field by field."""
     codes = {vp: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f", C.c_double: "d"}
     fmt = "".join(f"{t._length_}{codes[t._type_]}" if hasattr(t, "_length_") else codes[t] for _, t in cls._fields_)
     pack = struct.Struct("@" + fmt)
     assert pack.size <= C.sizeof(cls) < pack.size + 8  # the tail padding is the struct's own
-    pad = bytes(C.sizeof(cls) - pack.size)
-    return lambda *values: cls.from_buffer_copy(pack.pack(*values) + pad)
+    return pack.pack if pack.size == C.sizeof(cls) else struct.Struct(f"@{fmt}{C.sizeof(cls) - pack.size}x").pack
 
 
 def launch(fn, args, gpu: int) -> int:

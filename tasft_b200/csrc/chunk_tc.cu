@@ -722,7 +722,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       constexpr uint32_t fmt = kF16 ? 0u : 1u;
       constexpr uint32_t idesc_s = tc::make_idesc(128, 64, fmt, false);
       constexpr uint32_t idesc_o = tc::make_idesc(128, D, fmt, true);
-      const uint32_t q_addr = smem_u32(sQ);
+      // descriptors once; the address field counts 16-byte units and does not overflow
+      const uint64_t q_desc = tc::make_sdesc(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = tc::make_sdesc(smem_u32(smem + L::kStageOff + L::kKOff), 16, 1024);
+      const uint64_t v_desc = tc::make_sdesc(smem_u32(smem + L::kStageOff + L::kVOff), 64 * 128, 1024);
       int g = 0, tile = -1;
       bool ok = true, started = false;
       auto issue_s = [&](int gi) -> bool {
@@ -731,14 +734,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         // S(gi) overwrites P(gi - 2) in TMEM: P.V(gi - 2) was issued earlier by this thread, and
         // the MMAs of one thread run through the tensor pipe in issue order
         tc::tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + L::kStageOff + L::kKOff + kst * L::kKVTileBytes);
+        const uint64_t kd = k_desc + (uint32_t)(kst * (L::kKVTileBytes >> 4));
         const uint32_t dst = tS0 + st * 64;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t ad = tc::make_sdesc(q_addr + (kk >> 2) * 128 * 128 + (kk & 3) * 32, 16, 1024);
-          const uint64_t bd = tc::make_sdesc(k_addr + (kk >> 2) * 64 * 128 + (kk & 3) * 32, 16, 1024);
-          tc::mma_ss(dst, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc::mma_ss(dst, q_desc + (uint32_t)(((kk >> 2) * 128 * 128 + (kk & 3) * 32) >> 4),
+                     kd + (uint32_t)(((kk >> 2) * 64 * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
         tc::mma_commit(&s_full[st]);
         tc::mma_commit(&k_empty[kst]);
         return true;
@@ -769,13 +770,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int vst = gi % L::kRing;
           if (!mbar_wait(&v_full[vst], (gi / L::kRing) & 1)) { ok = false; break; }
           tc::tc_fence_after();
-          const uint32_t v_addr = smem_u32(smem + L::kStageOff + L::kVOff + vst * L::kKVTileBytes);
+          const uint64_t vd = v_desc + (uint32_t)(vst * (L::kKVTileBytes >> 4));
           const uint32_t p_tmem = tS0 + (gi & 1) * 64;
 #pragma unroll
-          for (int kk = 0; kk < kChunkBlk / 16; ++kk) {
-            const uint64_t bd = tc::make_sdesc(v_addr + kk * 16 * 128, 64 * 128, 1024);
-            tc::mma_ts(tO, p_tmem + kk * 8, bd, idesc_o, (started || kk > 0) ? 1u : 0u);
-          }
+          for (int kk = 0; kk < kChunkBlk / 16; ++kk)
+            tc::mma_ts(tO, p_tmem + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), idesc_o, (started || kk > 0) ? 1u : 0u);
           started = true;
           tc::mma_commit(&v_empty[vst]);
           tc::mma_commit(&pv_done[gi & 1]);
