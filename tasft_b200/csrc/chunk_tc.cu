@@ -290,6 +290,26 @@ __global__ void __launch_bounds__(kThreads, 2)
     // whole tiles would take rounds * widest; cut ones take `step`
     const int64_t rounds = (uint32_t)(count + G - 1) / (uint32_t)G;
     cutting = sh.may_cut && rounds * widest - step > (int64_t)kChunkMergeCost * kChunkBlk;
+    if (!cutting) {  // whole tiles: each CTA takes as many, one more here and there (weight 64 each)
+      total = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + lane;
+        int64_t w = 0;
+        if (b < a.B) {
+          int tiles;
+          if (sh.stride == 1) {
+            const int4 q4 = seqs[b];
+            tiles = chunk_tiles(sh, q4.y, q4.z - q4.y, q4.z);
+          } else {
+            tiles = chunk_seq(a, sh, b).tiles;
+          }
+          w = (int64_t)tiles * sh.units * kChunkBlk;
+        }
+        const int64_t upto = warp_scan64(w, lane);
+        if (b < a.B && (sh.stride == 1 || b % sh.stride == 0)) before[sh.stride == 1 ? b : b / sh.stride] = total + upto - w;
+        total += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
     __syncwarp();
   }
   tc::tc_fence_before();
@@ -323,8 +343,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       s.bad = false;
       return s;
     };
-    // The place at weight x, in Int arithmetic. Cuts within two blocks of a tile's end, or all
-    // where tiles stay whole, go to the nearer end.
+    auto weight = [&](const ChunkSeq& s, int i) -> int64_t { return cutting ? chunk_weight(sh, s, i) : kChunkBlk; };
+    auto weight_before = [&](const ChunkSeq& s, int i) -> int64_t {
+      return cutting ? chunk_weight_before(sh, s, i) : (int64_t)i * kChunkBlk;
+    };
+    // The place at weight x, in Int arithmetic. Cuts within two blocks of a tile's end go there.
     auto find = [&](auto zero, int64_t x64) -> ChunkCut {
       using Int = decltype(zero);
       ChunkCut c;
@@ -342,30 +365,30 @@ __global__ void __launch_bounds__(kThreads, 2)
       Int x = (Int)(x64 - before[bl]);
       c.b = bl * sh.stride;
       c.s = get_seq(c.b);
-      Int per = (Int)chunk_weight_before(sh, c.s, c.s.tiles);
+      Int per = (Int)weight_before(c.s, c.s.tiles);
       while (x >= per * (Int)sh.units) {  // sequences without new tokens have no weight
         x -= per * (Int)sh.units;
         c.s = get_seq(++c.b);
-        per = (Int)chunk_weight_before(sh, c.s, c.s.tiles);
+        per = (Int)weight_before(c.s, c.s.tiles);
       }
       c.unit = (int)(x / per);
       x -= (Int)c.unit * per;
-      if (sh.mode != 0) {
-        c.tile = (int)(x / (Int)(c.s.cost * kChunkBlk));
+      if (sh.mode != 0 || !cutting) {
+        c.tile = (int)(x / (Int)weight(c.s, 0));
       } else {  // the weights before tiles grow as t i^2 / 2 + (ctx + 63 + t / 2) i
         const float t = (float)sh.tpt, h = (float)(c.s.ctx + 63) + 0.5f * t;
         int i = (int)((sqrtf(h * h + 2.f * t * (float)x) - h) / t);
         i = max(0, min(i, c.s.tiles - 1));
-        while (i > 0 && (Int)chunk_weight_before(sh, c.s, i) > x) --i;
-        while (i + 1 < c.s.tiles && (Int)chunk_weight_before(sh, c.s, i + 1) <= x) ++i;
+        while (i > 0 && (Int)weight_before(c.s, i) > x) --i;
+        while (i + 1 < c.s.tiles && (Int)weight_before(c.s, i + 1) <= x) ++i;
         c.tile = i;
       }
-      c.rho = (int64_t)(x - (Int)chunk_weight_before(sh, c.s, c.tile));
-      c.w = chunk_weight(sh, c.s, c.tile);
-      const int64_t edge = cutting ? 2 * kChunkBlk : (c.w + 1) / 2;
-      if (c.rho < edge) {
+      c.rho = (int64_t)(x - (Int)weight_before(c.s, c.tile));
+      c.w = weight(c.s, c.tile);
+      constexpr int kEdge = 2 * kChunkBlk;
+      if (c.rho < kEdge) {  // (always, where tiles stay whole)
         c.rho = 0;
-      } else if (c.w - c.rho < edge || !cutting) {  // the start of the next tile
+      } else if (c.w - c.rho < kEdge) {  // the start of the next tile
         c.rho = 0;
         if (++c.tile == c.s.tiles) {
           c.tile = 0;
@@ -381,7 +404,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       return c;
     };
     // both ends at once, in the even and the odd lanes
-    const int64_t end_x = (int64_t)(blockIdx.x + (lane & 1)) * step;
+    const int64_t nth = blockIdx.x + (lane & 1);
+    const int64_t end_x = cutting ? nth * step : nth * (total / kChunkBlk) / (int64_t)gridDim.x * kChunkBlk;
     const ChunkCut end = total < (1ll << 31) ? find(0u, end_x) : find((int64_t)0, end_x);
     auto take = [&](int from_lane) -> ChunkCut {
       ChunkCut c;
