@@ -1362,10 +1362,12 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   int bound = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
   if (a.kept_idx && (int64_t)a.nb_w * 2 < bound) bound = a.nb_w * (sh.mode == 2 ? 2 : 1);
   sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
-  // One launch where cutting tiles gains nothing: the gain is at most the last round's idle share
-  // of a tile as long as can be, for as many tiles as the tokens fill (the device decides the rest).
+  // One launch where cutting tiles gains nothing (the device decides the rest). Tiles with lists
+  // take about as long as one another: the gain is the last round's idle share of the longest, for
+  // as many tiles as the tokens fill. Without lists they may differ by all their blocks.
   const int64_t G = 2 * sm_count(), tiles = ((int64_t)a.T / sh.tpt + a.B) * sh.units;
-  sh.may_cut = ((tiles + G - 1) / G * G - tiles) * bound > kChunkMergeCost * G;
+  sh.may_cut = sh.mode == 0 ? bound > kChunkMergeCost
+                            : ((tiles + G - 1) / G * G - tiles) * bound > kChunkMergeCost * G;
   if (!a.workspace || a.workspace_bytes < ws_layout(sh, a.D, (int)G).bytes) return TASFT_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count();
