@@ -20,7 +20,8 @@ struct ChunkShape {
   int capacity;   // tokens the block table can hold (max_pages * page_size)
   int rows;       // rows of a piece's partials
   int stride;     // sequences per entry of the table
-  int may_cut;    // 0: no tile is long enough to be cut
+  int may_cut;    // 0: cutting tiles gains nothing
+  int wide;       // rows of out on 32-byte boundaries
 };
 
 struct ChunkSeq {

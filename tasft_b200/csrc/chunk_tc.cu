@@ -84,6 +84,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
+// 32-byte store: a whole sector per lane, where rows lie far apart.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // One arrival for the warp: what its lanes did before is released by lane 0. (32 lanes that
 // arrive one by one on the same barrier take some 500 cycles.)
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -966,9 +973,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 pk[c] = kF16 ? tc::pack_f16x2(v0, v1) : tc::pack_bf16x2(v0, v1);
               }
-              uint4* dst = reinterpret_cast<uint4*>(orow + c0);
+              if (sh.wide) {
+                store32(orow + c0, pk);
+                store32(orow + c0 + 16, pk + 8);
+              } else {
+                uint4* dst = reinterpret_cast<uint4*>(orow + c0);
 #pragma unroll
-              for (int v = 0; v < 4; ++v) dst[v] = make_uint4(pk[4 * v], pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+                for (int v = 0; v < 4; ++v) dst[v] = make_uint4(pk[4 * v], pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+              }
             }
           }
         } else {
@@ -984,11 +996,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                   o[c] = __float_as_uint(nonfinite_of((code[((c0 + c) >> 4) * 128] >> (((c0 + c) & 15) * 2)) & 3, __uint_as_float(o[c])));
               }
               if (live) {
-                float4* dst = reinterpret_cast<float4*>(ws.o + prow * D + c0);
 #pragma unroll
-                for (int v = 0; v < 8; ++v)
-                  dst[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
-                                       __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
+                for (int v = 0; v < 4; ++v) store32(ws.o + prow * D + c0 + 8 * v, o + 8 * v);
               }
             }
           }
@@ -1361,6 +1370,8 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   // most blocks a tile visits
   int bound = (sh.capacity + kChunkBlk - 1) / kChunkBlk;
   if (a.kept_idx && (int64_t)a.nb_w * 2 < bound) bound = a.nb_w * (sh.mode == 2 ? 2 : 1);
+  // 32-byte stores of out's rows
+  sh.wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.o_stride[0] % 16 == 0 && a.o_stride[1] % 16 == 0;
   sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
   // One launch where cutting tiles gains nothing (the device decides the rest). Tiles with lists
   // take about as long as one another: the gain is the last round's idle share of the longest, for
