@@ -672,80 +672,81 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 0) {
     // ================= producer =================
+    // The lanes share the copies of a tile, one each: eight for pages of 16 tokens at D 128.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (lane == 0) {
       tc::prefetch_tmap(&tmq);
       tc::prefetch_tmap(&tmk);
       tc::prefetch_tmap(&tmv);
-      const int nsub = max(1, kChunkBlk / a.page_size), sub_rows = min(kChunkBlk, a.page_size);
-      const uint32_t q_bytes = sh.mode == 2 ? 0 : (uint32_t)(L::kChunks * sh.hpt * sh.tpt * 128);
-      const int all_pages = (1 << nsub) - 1;
-      int gk = 0, gv = 0, tile = 0, looks = 0;  // K and V tiles asked for, tiles, V tiles for warp 3
-      bool ok = true;
-      for (int u = 0; ok; ++u) {
-        const int lb = u & 1;
-        if (!mbar_wait(&list_full[lb], (u >> 1) & 1)) { ok = false; break; }
-        const Work& w = works[lb];
-        const int n = w.n;
-        if (n < 0) break;
-        if (w.first) {
-          if (tile >= 1 && !mbar_wait(q_empty, (tile - 1) & 1)) { ok = false; break; }
-          if (sh.mode == 2) {
-            const int nv = (w.valid[0] ? 1 : 0) + (w.valid[1] ? 1 : 0);
-            mbar_arrive_expect_tx(q_full, nv * L::kChunks * 64 * 128);
-            for (int x = 0; x < 2; ++x) {
-              if (!w.valid[x]) continue;
-              for (int c = 0; c < L::kChunks; ++c)
-                tc::tma_load_4d(sQ + c * 128 * 128 + x * 64 * 128, &tmq, c * 64, w.head[x], w.row[x], 0, q_full);
-            }
-          } else {
-            mbar_arrive_expect_tx(q_full, q_bytes);
-            for (int c = 0; c < L::kChunks; ++c)
-              tc::tma_load_4d(sQ + c * 128 * 128, &tmq, c * 64, w.head[0], w.row[0], 0, q_full);
-          }
-          ++tile;
-        }
-        const int32_t* list = lists + lb * kSeg;
-        const int32_t* pgs = reinterpret_cast<const int32_t*>(pages + lb * kSeg);
-        const Look look(w, sh);
-        // one entry's K or V: the share of each page it has, into the stage's rows
-        auto load = [&](int gi, int j, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off) -> bool {
-          const int st = gi % L::kRing;
-          if (gi >= L::kRing && !mbar_wait(&empty[st], (gi / L::kRing - 1) & 1)) return false;
-          const int e = list[j], have = (e >> kKbBits) & 15, kbase = (e & kKbMask) * kChunkBlk;
-          const int in_page = a.page_size > kChunkBlk ? ((e & kKbMask) & 1) * kChunkBlk : 0;
-          uint8_t* dst = smem + L::kStageOff + off + st * L::kKVTileBytes;
-          uint64_t* bar = &full[st];
-          if (full == v_full && look.wanted(e, kbase, have, all_pages, w.len)) bar = &v_look[looks++ % L::kRing];
-          mbar_arrive_expect_tx(bar, (uint32_t)(__popc(have) * L::kChunks * sub_rows * 128));
-          for (int x = 0; x < nsub; ++x) {
-            if (!((have >> x) & 1)) continue;
-            for (int c = 0; c < L::kChunks; ++c)
-              tc::tma_load_4d(dst + c * 64 * 128 + x * sub_rows * 128, map, c * 64, w.hk, in_page, pgs[4 * j + x], bar);
-          }
-          return true;
-        };
-        // K(j) then V(j-1): the order the MMA warp consumes them
-        for (int j = 0; ok && j <= n && n > 0; ++j) {
-          if (j < n) {
-            ok = load(gk, j, &tmk, k_full, k_empty, L::kKOff);
-            if (ok) ++gk;
-          }
-          if (ok && j >= 1) {
-            ok = load(gv, j - 1, &tmv, v_full, v_empty, L::kVOff);
-            if (ok) ++gv;
-          }
-        }
-        // the softmax warps may be through with the segment while its last V is not on its way yet
-        if (ok) mbar_arrive(&list_empty[lb]);
-      }
-      if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 10));
-      // do not leave while copies into shared memory are in flight, after a timeout either
-      if (tile > 0) mbar_wait(q_full, (tile - 1) & 1);
-      for (int i = max(0, gk - L::kRing); i < gk; ++i) mbar_wait(&k_full[i % L::kRing], (i / L::kRing) & 1);
-      for (int i = max(0, looks - L::kRing); i < looks; ++i) mbar_wait(&v_look[i % L::kRing], (i / L::kRing) & 1);
-      for (int i = max(0, gv - L::kRing); i < gv; ++i) mbar_wait(&v_full[i % L::kRing], (i / L::kRing) & 1);
     }
+    const int nsub = max(1, kChunkBlk / a.page_size), sub_rows = min(kChunkBlk, a.page_size);
+    const uint32_t q_bytes = sh.mode == 2 ? 0 : (uint32_t)(L::kChunks * sh.hpt * sh.tpt * 128);
+    const int all_pages = (1 << nsub) - 1;
+    const int my_c = lane % L::kChunks, my_x = lane / L::kChunks;  // the lane's column chunk and page (or slot of Q)
+    int gk = 0, gv = 0, tile = 0, looks = 0;  // K and V tiles asked for, tiles, V tiles for warp 3
+    bool ok = true;
+    for (int u = 0; ok; ++u) {
+      const int lb = u & 1;
+      if (!warp_wait(&list_full[lb], (u >> 1) & 1)) { ok = false; break; }
+      const Work& w = works[lb];
+      const int n = w.n;
+      if (n < 0) break;
+      if (w.first) {
+        if (tile >= 1 && !warp_wait(q_empty, (tile - 1) & 1)) { ok = false; break; }
+        if (lane == 0)
+          mbar_arrive_expect_tx(q_full, sh.mode == 2 ? ((w.valid[0] ? 1 : 0) + (w.valid[1] ? 1 : 0)) * L::kChunks * 64 * 128
+                                                     : q_bytes);
+        __syncwarp();
+        if (sh.mode == 2) {
+          if (my_x < 2 && w.valid[my_x])
+            tc::tma_load_4d(sQ + my_c * 128 * 128 + my_x * 64 * 128, &tmq, my_c * 64, w.head[my_x], w.row[my_x], 0, q_full);
+        } else if (my_x == 0) {
+          tc::tma_load_4d(sQ + my_c * 128 * 128, &tmq, my_c * 64, w.head[0], w.row[0], 0, q_full);
+        }
+        ++tile;
+      }
+      const int32_t* list = lists + lb * kSeg;
+      const int32_t* pgs = reinterpret_cast<const int32_t*>(pages + lb * kSeg);
+      const Look look(w, sh);
+      const int hk = w.hk, len = w.len;
+      // one entry's K or V: the share of each page it has, into the stage's rows
+      auto load = [&](int gi, int j, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off) -> bool {
+        const int st = gi % L::kRing;
+        const int e = list[j], have = (e >> kKbBits) & 15, kbase = (e & kKbMask) * kChunkBlk;
+        const int page = pgs[4 * j + (my_x & 3)];
+        const int in_page = a.page_size > kChunkBlk ? ((e & kKbMask) & 1) * kChunkBlk : 0;
+        uint8_t* dst = smem + L::kStageOff + off + st * L::kKVTileBytes;
+        uint64_t* bar = &full[st];
+        if (full == v_full && look.wanted(e, kbase, have, all_pages, len)) bar = &v_look[looks++ % L::kRing];
+        if (gi >= L::kRing && !warp_wait(&empty[st], (gi / L::kRing - 1) & 1)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(__popc(have) * L::kChunks * sub_rows * 128));
+        __syncwarp();
+        if (my_x < nsub && ((have >> my_x) & 1))
+          tc::tma_load_4d(dst + my_c * 64 * 128 + my_x * sub_rows * 128, map, my_c * 64, hk, in_page, page, bar);
+        return true;
+      };
+      // K(j) then V(j-1): the order the MMA warp consumes them
+      for (int j = 0; ok && j <= n && n > 0; ++j) {
+        if (j < n) {
+          ok = load(gk, j, &tmk, k_full, k_empty, L::kKOff);
+          if (ok) ++gk;
+        }
+        if (ok && j >= 1) {
+          ok = load(gv, j - 1, &tmv, v_full, v_empty, L::kVOff);
+          if (ok) ++gv;
+        }
+      }
+      // the softmax warps may be through with the segment while its last V is not on its way yet
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive(&list_empty[lb]);
+    }
+    if (!ok) set_err(a.err, TASFT_DEVERR_TIMEOUT | (1 << 10));
+    // do not leave while copies into shared memory are in flight, after a timeout either (a look that
+    // was counted but not asked for then only runs out its wait)
+    if (tile > 0) warp_wait(q_full, (tile - 1) & 1);
+    for (int i = max(0, gk - L::kRing); i < gk; ++i) warp_wait(&k_full[i % L::kRing], (i / L::kRing) & 1);
+    for (int i = max(0, looks - L::kRing); i < looks; ++i) warp_wait(&v_look[i % L::kRing], (i / L::kRing) & 1);
+    for (int i = max(0, gv - L::kRing); i < gv; ++i) warp_wait(&v_full[i % L::kRing], (i / L::kRing) & 1);
   } else if (warp == 1) {
     // ================= MMA issuer =================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
