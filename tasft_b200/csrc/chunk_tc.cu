@@ -861,13 +861,21 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int entry = list[j];
         const int kbase = (entry & kKbMask) * kChunkBlk;
         const int have = (entry >> kKbBits) & 15;
-        if (any_live) {
+        // keys this row may see: up to its own position
+        int lim = qpos - kbase + 1;
+        if (!live || !((entry >> (kKbBits + 4 + slot)) & 1)) lim = 0;
+        lim = max(0, min(lim, kChunkBlk));
+        if (!__any_sync(0xffffffffu, lim > 0)) {
+          if (any_live) {  // no row of the warp sees a key of this block: p = 0
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pk[c] = 0u;
+            tc::tmem_st32(tS0 + (gi & 1) * 64 + lane_off, pk);
+            tc::tmem_wait_st();
+          }
+        } else {
           uint32_t sraw[64];
           tc::tmem_ld64_sync(tS0 + (gi & 1) * 64 + lane_off, sraw);
-          // keys this row may see: up to its own position
-          int lim = qpos - kbase + 1;
-          if (!live || !((entry >> (kKbBits + 4 + slot)) & 1)) lim = 0;
-          lim = max(0, min(lim, kChunkBlk));
           float sv[64];
 #pragma unroll
           for (int c = 0; c < 64; ++c) sv[c] = __uint_as_float(sraw[c]);
