@@ -879,18 +879,20 @@ __global__ void __launch_bounds__(kThreads, 2)
           float sv[64];
 #pragma unroll
           for (int c = 0; c < 64; ++c) sv[c] = __uint_as_float(sraw[c]);
-          if (__any_sync(0xffffffffu, lim < kChunkBlk)) {
+          if (__any_sync(0xffffffffu, lim < kChunkBlk) || have != all_pages) {
+            uint64_t seen = lim == kChunkBlk ? ~0ull : (1ull << lim) - 1;
+            if (have != all_pages) {  // keys of a page that is not there
+              uint64_t keys = 0;
+              for (int x = 0; x * sub_rows < kChunkBlk; ++x)
+                if ((have >> x) & 1) keys |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
+              seen &= keys;
+            }
+            const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c >= lim) sv[c] = -INFINITY;
-          }
-          if (have != all_pages) {  // keys of a page that is not there
-            uint64_t seen = 0;
-            for (int x = 0; x * sub_rows < kChunkBlk; ++x)
-              if ((have >> x) & 1) seen |= (sub_rows == 64 ? ~0ull : (1ull << sub_rows) - 1) << (x * sub_rows & 63);
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (!((seen >> c) & 1)) sv[c] = -INFINITY;
+            for (int c = 0; c < 32; ++c) {
+              if (!((s0 >> c) & 1)) sv[c] = -INFINITY;
+              if (!((s1 >> c) & 1)) sv[32 + c] = -INFINITY;
+            }
           }
           float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
