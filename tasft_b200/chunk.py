@@ -159,7 +159,7 @@ def rope_append_paged(
     by ``attention_scaling``. ``max_new``: most new tokens of a sequence. With ``pooled_k`` (fp32
     ``[B, Hk, NBk, D]``, updated in place: the mean of every key block that got new tokens) also
     computes the means of the new queries. Returns ``(q, pooled_q)``: rotated q (``out``, which may
-    be q itself) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for
+    be q itself; rows outside all sequences are not written) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for
     :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
     256. The packed, paged counterpart of :func:`qkv_rope_pool`, which takes cos and sin as tables."""
     name = "rope_append_paged"
@@ -300,11 +300,11 @@ def bsa_chunk_paged(
     q ``[T, Hq, D]``, pages ``[num_pages, page_size, Hk, D]`` with the new keys and values already
     in them (:func:`rope_append_paged`), ``kept`` lists ``[B, Hk or Hq, NBq, W]`` with at least
     ``chunk_rows(max_new)`` rows, ascending. ``scale`` defaults to ``1 / sqrt(D)``. Returns
-    ``[T, Hq, D]`` (``out``; rows outside all sequences stay as they were); a token with nothing
-    kept gets 0. ``err``: optional int32 error word, see ``include/tasft_b200.h``. bf16 / f16, D 64
-    or 128, page size 16, 32, 64 or 128. What the cache holds from ``kv_len`` on, or in blocks no
-    list keeps, is never read into the result; a non-finite value of a kept block's own token
-    spreads as the softmax formula has it. Beside :func:`bsa_decode_paged` (one token per sequence) and
+    ``[T, Hq, D]`` (``out``; rows outside all sequences stay as they were, undefined in a new
+    tensor); a token with nothing kept gets 0. ``err``: optional int32 error word, see ``include/tasft_b200.h``. bf16 / f16, D 64
+    or 128, page size 16, 32, 64 or 128. What the cache holds from ``kv_len`` on, behind a
+    token's own position or in blocks its list does not keep never reaches its row, infinities
+    and NaN neither. Beside :func:`bsa_decode_paged` (one token per sequence) and
     :meth:`BlockSparseFlashAttention.forward_varlen` (no cache)."""
     name = "bsa_chunk_paged"
     gpu, qs, ks = q.get_device(), q.shape, k_pages.shape
@@ -345,6 +345,9 @@ def bsa_chunk_paged(
         q = q.contiguous()
         st = q.stride()
     lib = L.lib()
+    if gpu != torch._C._cuda_getDevice():  # the workspace is sized for the current device
+        with torch.cuda.device(gpu):
+            return bsa_chunk_paged(q, k_pages, v_pages, table, cu, kvl, max_new, kept, block, scale=scale, out=out, err=err)
     nbytes = lib.tasft_chunk_workspace_size(B, T, Hq, Hk, D, max_new, hm)
     if nbytes < 0:
         L.check(int(nbytes), "tasft_chunk_workspace_size", shape=[B, T, Hq, Hk, D])

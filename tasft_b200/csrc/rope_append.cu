@@ -286,7 +286,7 @@ extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_s
   if (!ap) return TASFT_ERR_INVALID_ARG;
   tasft_rope_append_args a = *ap;
   // strides of axes of length one say nothing
-  if (a.T == 1) a.q_stride[0] = a.k_in_stride[0] = a.v_in_stride[0] = a.o_stride[0] = 0;
+  if (a.T <= 1) a.q_stride[0] = a.k_in_stride[0] = a.v_in_stride[0] = a.o_stride[0] = 0;
   if (a.Hq == 1) a.q_stride[1] = a.o_stride[1] = 0;
   if (a.Hk == 1) a.k_in_stride[1] = a.v_in_stride[1] = a.k_stride[2] = a.v_stride[2] = 0;
   if (a.num_pages == 1) a.k_stride[0] = a.v_stride[0] = 0;
@@ -305,8 +305,8 @@ extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_s
   const int per16 = 16 / elem_size(a.dtype);
   // 16-byte column pairs: whole heads and the rotated part are multiples of two of them
   if (a.D % (2 * per16) || a.rot % (2 * per16) || a.D > 256) return TASFT_ERR_UNSUPPORTED;
-  if (a.T == 0) return TASFT_OK;
-  if (!a.q || !a.k || !a.v || !a.q_out) return TASFT_ERR_INVALID_ARG;
+  if (a.T == 0 && !a.pooled_q) return TASFT_OK;
+  if (a.T > 0 && (!a.q || !a.k || !a.v || !a.q_out)) return TASFT_ERR_INVALID_ARG;
   if (!aligned16(a.pooled_q) || !aligned16(a.pooled_k)) return TASFT_ERR_UNSUPPORTED;
   if (!rows_ok(a.q, a.q_stride, 2, per16) || !rows_ok(a.k, a.k_in_stride, 2, per16) ||
       !rows_ok(a.v, a.v_in_stride, 2, per16) || !rows_ok(a.q_out, a.o_stride, 2, per16) ||

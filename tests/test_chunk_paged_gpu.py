@@ -88,6 +88,24 @@ def test_many_sequences_and_empty_ones():
 
 
 @pytest.mark.parametrize("lists", [None, "kv", "q"])
+def test_more_sequences_than_the_table_with_tiles_in_pieces(lists):
+    """Two sequences per entry of the kernel's table, a few of them long enough to be cut."""
+    new = [0] * 290
+    ctx = [0] * 290
+    for b, (n, c) in {3: (1, 15000), 4: (40, 70), 100: (70, 9000), 101: (1, 1), 288: (2, 20000), 289: (1, 63)}.items():
+        new[b], ctx[b] = n, c
+    spec = None if lists is None else ((2 if lists == "kv" else 8), 0.7, True, 0.0)
+    check(new, ctx, 8, 2, 64, 64, torch.bfloat16, spec, seed=18)
+
+
+@pytest.mark.parametrize("n,ctx", [(2048, 0), (700, 5000), (1, 7000)])
+@pytest.mark.parametrize("Hq,Hk", [(4, 4), (7, 1)])
+def test_tiles_of_many_lengths_in_pieces(n, ctx, Hq, Hk):
+    check([n], [ctx], Hq, Hk, 128, 32, torch.float16, seed=19)
+    check([n], [ctx], Hq, Hk, 128, 32, torch.float16, (Hk, 0.8, True, 0.05), seed=20)
+
+
+@pytest.mark.parametrize("lists", [None, "kv", "q"])
 def test_long_context_is_split(lists):
     spec = None if lists is None else ((4 if lists == "kv" else 28), 0.6, True, 0.0)
     check([1], [32767], 28, 4, 128, 16, torch.bfloat16, spec, seed=5)
@@ -257,6 +275,16 @@ def test_a_query_that_is_nan_gives_nan():
     assert torch.isnan(out[7, 2]).all()
     out[7, 2] = good[7, 2]
     assert torch.equal(out, good)
+
+
+def test_no_tokens_and_odd_strides_of_single_axes():
+    q, kp, vp, table, cu, kv_len, g = case([3, 2], [40, 9], 4, 1, 64, 16, torch.bfloat16, 21)
+    none = T.bsa_chunk_paged(q[:0], kp, vp, table, torch.zeros_like(cu), kv_len, 3)
+    assert none.shape == (0, 4, 64)
+    want = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, 3)
+    one = torch.as_strided(q[4:5], (1, 4, 64), (3, 64, 1))  # one token: its stride says nothing
+    got = T.bsa_chunk_paged(one, kp, vp, table[1:], torch.tensor([0, 1], dtype=torch.int32, device=DEV), kv_len[1:], 1)
+    assert torch.equal(got, want[4:5])
 
 
 def test_graph_replay_follows_its_inputs():

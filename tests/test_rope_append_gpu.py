@@ -130,6 +130,16 @@ def test_pieces_equal_the_whole():
     assert torch.allclose(m1, m2, rtol=0, atol=65 * 2.0 ** -24 * 4)
 
 
+def test_no_tokens_give_means_of_zero():
+    rows, kp, vp, table, cu, kv_len, freq, f = case([4], [30], 4, 2, 64, 16, torch.bfloat16, 64, seed=7)
+    means = torch.full((1, 2, 2, 64), 5.0, device=DEV)
+    k0 = kp.clone()
+    out, pooled_q = T.rope_append_paged(rows[:0, :4], rows[:0, 4:6], rows[:0, 6:], freq, kp, vp, table, torch.zeros_like(cu),
+                                        kv_len, 3, pooled_k=means)
+    assert out.shape == (0, 4, 64) and (pooled_q == 0).all() and (means == 5).all()
+    assert torch.equal(kp.nan_to_num(9), k0.nan_to_num(9))
+
+
 def test_in_place_and_fp32_frequencies():
     rows, kp, vp, table, cu, kv_len, freq, f = case([90], [10], 4, 4, 64, 16, torch.float16, 64, seed=5)
     q = rows[:, :4].contiguous()
