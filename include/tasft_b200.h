@@ -21,6 +21,10 @@
  *   tasft_mask_from_scores     soft >= tau (+ tril)       tasft/modules/attn_gate.py:466-477
  *   tasft_qkv_rope_pool        _prepare_qkv head split + rotary + the gate's pooling
  *                              tasft/modules/tasft_attention.py:615-742, attn_gate.py:351-375
+ *   tasft_rope_append_paged    (none: the paged, packed form of tasft_qkv_rope_pool)
+ *   tasft_select_blocks        (none: top-scored blocks; the reference keeps by threshold)
+ *   tasft_bsa_chunk_paged_fwd  (none: the reference's vLLM prefill has no cache behind it,
+ *                              tasft/inference/vllm_patch.py:172-196)
  *   tasft_mask_to_kept         bool mask & block tril     tasft/kernels/block_sparse_fa.py:497-508
  *   tasft_calibrate_tau        the weight-norm estimate of per-layer sparsity
  *                                                         tasft/bundle/export.py:327-360
@@ -371,7 +375,8 @@ TASFT_API int tasft_bsa_decode_paged_fwd(const tasft_paged_decode_args* args, ta
  * strides of whole 16 bytes. Reported in *err without a fault: TASFT_DEVERR_INDEX (a page or
  * kept block out of range: skipped; a sequence whose lengths do not fit T, max_q, each other
  * or the table: its rows are left out), TASFT_DEVERR_ORDER (a list that does not ascend: the
- * entry is skipped). Cache rows from kv_len on are never used, whatever they hold. */
+ * entry is skipped). Cache rows from kv_len on, and
+ * values of K and V that are not finite behind a token's mask, never reach its row. */
 typedef struct {
   const void* q;            /* [T, Hq, D] */
   const void* k_pages;      /* [num_pages, page_size, Hk, D] */

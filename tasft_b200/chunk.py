@@ -201,7 +201,8 @@ def rope_append_paged(
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != qs or out.dtype is not dtype or out.get_device() != gpu or out.stride(2) != 1:
         raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
-    (q, qt), (k, kt), (v, vt) = _rows(q), _rows(k), _rows(v)
+    per16 = 16 // dtype.itemsize
+    (q, qt), (k, kt), (v, vt) = _rows(q, per16), _rows(k, per16), _rows(v, per16)
     freq = inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
     args = _rope_args(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
@@ -215,11 +216,11 @@ def rope_append_paged(
     return out, pooled_q
 
 
-def _rows(x: torch.Tensor):
-    """x with contiguous columns, and its strides."""
+def _rows(x: torch.Tensor, per16: int):
+    """x as rows on 16-byte boundaries with contiguous columns (a copy where it is not), and its strides."""
     st = x.stride()
-    if st[2] != 1:
-        x = x.contiguous()
+    if st[2] != 1 or st[0] % per16 or st[1] % per16 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
         st = x.stride()
     return x, st
 
@@ -340,10 +341,7 @@ def bsa_chunk_paged(
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != qs or out.dtype is not q.dtype or out.get_device() != gpu or out.stride(2) != 1:
         raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
-    st = q.stride()
-    if st[2] != 1 or st[0] % 8 or st[1] % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-        st = q.stride()
+    q, st = _rows(q, 8)
     lib = L.lib()
     if gpu != torch._C._cuda_getDevice():  # the workspace is sized for the current device
         with torch.cuda.device(gpu):

@@ -285,6 +285,10 @@ def test_no_tokens_and_odd_strides_of_single_axes():
     one = torch.as_strided(q[4:5], (1, 4, 64), (3, 64, 1))  # one token: its stride says nothing
     got = T.bsa_chunk_paged(one, kp, vp, table[1:], torch.tensor([0, 1], dtype=torch.int32, device=DEV), kv_len[1:], 1)
     assert torch.equal(got, want[4:5])
+    flat = torch.empty(q.numel() + 1, device=DEV, dtype=q.dtype)
+    off = flat[1:].view(q.shape)  # not on a 16-byte boundary
+    off.copy_(q)
+    assert torch.equal(T.bsa_chunk_paged(off, kp, vp, table, cu, kv_len, 3), want)
 
 
 def test_graph_replay_follows_its_inputs():

@@ -147,6 +147,11 @@ def test_in_place_and_fp32_frequencies():
     assert none is None
     got, _ = T.rope_append_paged(q, rows[:, 4:8], rows[:, 8:], freq.float(), kp, vp, table, cu, kv_len, 90, out=q)
     assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    flat = torch.empty(rows.numel() + 1, device=DEV, dtype=rows.dtype)
+    off = flat[1:].view(rows.shape)  # not on a 16-byte boundary
+    off.copy_(rows)
+    again, _ = T.rope_append_paged(off[:, :4], off[:, 4:8], off[:, 8:], freq.float(), kp, vp, table, cu, kv_len, 90)
+    assert torch.equal(again, want)
 
 
 def test_bad_pages_and_sequences_write_nothing():
