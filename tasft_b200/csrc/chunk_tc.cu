@@ -15,7 +15,7 @@
 //      two lists and each entry says which slots keep it
 // Persistent CTAs (2 per SM, 256 threads) share the work evenly: all tiles in a row, weighted by
 // the blocks they visit, are cut into as many equal lengths as there are CTAs, through the middle
-// of tiles where that gains more than the merge costs (chunk_cut). A tile cut into pieces leaves
+// of tiles where that gains more than the merge costs (ChunkCut). A tile cut into pieces leaves
 // each piece's (m, l, O) in the workspace and chunk_merge_kernel joins them. Every CTA computes
 // the same cuts from cu_seqlens and kv_len, so the host needs neither. A CTA takes its length from
 // the back: the piece at its end starts at block 0 and the one at its start ends at the last, so

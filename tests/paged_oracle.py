@@ -113,7 +113,7 @@ def attend_bound(o, a, dtype, keys):
     return t
 
 
-def choose(scores, hk, new, ctx, top_k, tau=None, first=1, local=1, width=None):
+def choose(scores, hk, new, ctx, top_k, tau=None, first=1, local=1, width=None, block=BLK):
     """Kept lists from scores, by sorting (score, lowest index first) row by row."""
     B, Hq, rows, nbk = scores.shape
     width = min(nbk, max(top_k, first + local)) if width is None else width
@@ -122,8 +122,8 @@ def choose(scores, hk, new, ctx, top_k, tau=None, first=1, local=1, width=None):
     s = scores.double().cpu().view(B, hk, Hq // hk, rows, nbk)
     s = torch.where(torch.isnan(s), -math.inf, s).amax(2)
     for b, (n, c) in enumerate(zip(new, ctx)):
-        for i in range((c + n - 1) // BLK - c // BLK + 1 if n else 0):
-            mine = c // BLK + i
+        for i in range((c + n - 1) // block - c // block + 1 if n else 0):
+            mine = c // block + i
             forced = sorted(set(range(min(first, mine + 1))) | set(range(max(0, mine + 1 - local), mine + 1)))
             for h in range(hk):
                 row = s[b, h, i].tolist()

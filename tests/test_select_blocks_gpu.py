@@ -59,6 +59,14 @@ def test_forced_blocks(first, local, top_k):
     check(scores(2, 2, 6, 250, 3), 1, [290, 1], [3000, 250 * 64 - 1], top_k, first=first, local=local)
 
 
+@pytest.mark.parametrize("block,nbk", [(32, 40), (128, 300), (1, 600)])
+def test_other_block_sizes(block, nbk):
+    new, ctx = [3 * block, 1, 2], [nbk * block - 3 * block, 5 * block, 0]
+    check(scores(3, 6, 4, nbk, 11), 3, new, ctx, 6, block=block)
+    with pytest.raises(T.KernelError):
+        T.select_blocks(scores(1, 1, 1, 8), 1, *batch([1], [5]), 3, block=48)
+
+
 def test_masked_and_odd_scores():
     s = scores(1, 2, 1, 200, 4)
     s[:, 0, :, 5:90] = -math.inf
