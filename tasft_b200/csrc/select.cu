@@ -19,12 +19,10 @@
 namespace tasft {
 namespace {
 
-// fp32 -> uint32 of the same order (-inf lowest, NaN as -inf; -0 and +0 alike)
+// fp32 (not NaN) -> uint32 of the same order, -0 and +0 alike
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (!(x == x)) x = -INFINITY;
-  if (x == 0.f) x = 0.f;
-  const uint32_t u = __float_as_uint(x);
-  return (u >> 31) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 constexpr uint32_t kNever = 0x007fffffu;  // ordered(-inf): never chosen; below every other score
 
@@ -34,7 +32,8 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
   constexpr int kWords = kT * kV / 32;
   constexpr int kRowsPerCta = kT == 32 ? 4 : 1;
   __shared__ uint32_t bits_[kRowsPerCta][2 * kWords];  // above the threshold, at it
-  __shared__ int32_t place_[kRowsPerCta][kWords + 1];
+  __shared__ uint2 kept_[kRowsPerCta][kWords];  // the kept bits of a word, and the place of its first
+  __shared__ int32_t total_[kRowsPerCta];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = kT == 32 ? warp : 0, t = kT == 32 ? lane : threadIdx.x;
   // one CTA per row of a (row, kv-head, sequence) grid, or four consecutive rows per CTA
@@ -53,7 +52,7 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
   const int64_t row = ((int64_t)b * a.Hk + hk) * a.NBq + i;
   uint32_t* above = bits_[sub];
   uint32_t* at = above + kWords;
-  int32_t* place = place_[sub];
+  uint2* kept = kept_[sub];
   int32_t* idx = a.kept_idx + row * a.width;
   const int grp = a.Hq / a.Hk;
 
@@ -159,6 +158,7 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
         int top = hi == lo ? 0 : 32 - __clz(hi ^ lo);  // bits [0, top) are open
         thr = top == 32 ? 0u : hi >> top << top;
         quota = INT32_MAX;
+        bool first_digit = true;
         while (true) {
           if (top == 0) {  // all open keys are thr itself
             quota = left;
@@ -167,10 +167,16 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
           const int shift = max(0, top - 8);
           for (int i = t; i < 256; i += kT) hist[i] = 0;
           __syncthreads();
+          if (first_digit) {  // every key is open
 #pragma unroll
-          for (int v = 0; v < kV; ++v)
-            if (key[v] && (top == 32 || key[v] >> top == thr >> top))
-              atomicAdd(&hist[(key[v] >> shift) & ((1u << (top - shift)) - 1u)], 1);
+            for (int v = 0; v < kV; ++v)
+              if (key[v]) atomicAdd(&hist[(key[v] >> shift) & ((1u << (top - shift)) - 1u)], 1);
+          } else {
+#pragma unroll
+            for (int v = 0; v < kV; ++v)
+              if (key[v] >> top == thr >> top) atomicAdd(&hist[(key[v] >> shift) & ((1u << (top - shift)) - 1u)], 1);
+          }
+          first_digit = false;
           __syncthreads();
           // the digit in which the count from the top reaches `left` (256 threads or the first 128,
           // two digits each)
@@ -212,16 +218,15 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
   }
   // ---- bits: always kept or above the threshold; at the threshold, where not all of those are ----
   const bool all = quota == INT32_MAX;
+  const uint32_t from = want == 0 ? 0xffffffffu : all ? thr : thr + 1;  // scores are below the top value
 #pragma unroll
   for (int v = 0; v < kV; ++v) {
     const int j = v * kT + t;
-    const bool forced = j < lead || (j >= tail && j <= mine);
-    const bool up = want > 0 && (all ? key[v] >= thr : key[v] > thr);
-    const unsigned wa = __ballot_sync(0xffffffffu, forced || up);
-    const unsigned we = __ballot_sync(0xffffffffu, want > 0 && !all && key[v] == thr);
-    if (lane == 0) {
-      above[(v * kT + t) >> 5] = wa;
-      at[(v * kT + t) >> 5] = we;
+    const unsigned wa = __ballot_sync(0xffffffffu, key[v] >= from || j < lead || (j >= tail && j <= mine));
+    if (lane == 0) above[(v * kT + t) >> 5] = wa;
+    if (!all) {
+      const unsigned we = __ballot_sync(0xffffffffu, key[v] == thr);
+      if (lane == 0) at[(v * kT + t) >> 5] = we;
     }
   }
   if constexpr (kT > 32) __syncthreads();
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
     int ties = quota, out = 0;
     for (int w0 = 0; w0 < kWords; w0 += 32) {
       const int w = w0 + lane;
-      uint32_t e = w < kWords ? at[w] : 0u, m = w < kWords ? above[w] : 0u;
+      uint32_t e = !all && w < kWords ? at[w] : 0u, m = w < kWords ? above[w] : 0u;
       const int ne = __popc(e);
       int pre = ne;
 #pragma unroll
@@ -257,14 +262,11 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
         const int x = __shfl_up_sync(0xffffffffu, pk, o);
         if (lane >= o) pk += x;
       }
-      if (w < kWords) {
-        above[w] = m;
-        place[w] = out + pk - nk;
-      }
+      if (w < kWords) kept[w] = make_uint2(m, out + pk - nk);
       out += __shfl_sync(0xffffffffu, pk, 31);
     }
     if (lane == 0) {
-      place[kWords] = out;
+      total_[sub] = out;
       a.kept_cnt[row] = out;
     }
   }
@@ -273,10 +275,10 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
 #pragma unroll
   for (int v = 0; v < kV; ++v) {
     const int j = v * kT + t;
-    const uint32_t m = above[j >> 5];
-    if ((m >> lane) & 1) idx[place[j >> 5] + __popc(m & ((1u << lane) - 1u))] = j;
+    const uint2 m = kept[j >> 5];
+    if ((m.x >> lane) & 1) idx[m.y + __popc(m.x & ((1u << lane) - 1u))] = j;
   }
-  for (int j = place[kWords] + t; j < a.width; j += kT) idx[j] = -1;
+  for (int j = total_[sub] + t; j < a.width; j += kT) idx[j] = -1;
 }
 
 template <int kT, int kV>
