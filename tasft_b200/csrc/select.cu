@@ -12,8 +12,8 @@
 //
 // kT threads per row, kV values per thread (value v of thread t is block v * kT + t, so loads
 // are coalesced and a warp's ballot is one word of the bit rows). The scores are read once, 64 MB
-// for 2064 rows of up to 2048 blocks and 7 heads: 24.5 us on a B200 (9.8 at the copy rate), bound by
-// issue (some 1,100 instructions a warp) and the chain of loads and barriers; 512 short rows 5 us.
+// for 2064 rows of up to 2048 blocks and 7 heads: 25 us on a B200 (9.8 at the copy rate), bound by
+// issue (1,067 instructions a warp, slots 61% busy) and the chain of loads and barriers; 512 short rows 5 us.
 #include "common.cuh"
 
 namespace tasft {
