@@ -1367,7 +1367,7 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   if (!a.cu_seqlens || !a.kv_len || !a.block_table || !a.k_pages || !a.v_pages) return TASFT_ERR_INVALID_ARG;
   if (a.k_stride[3] != 1 || a.v_stride[3] != 1) return TASFT_ERR_INVALID_ARG;
   if (a.kept_idx) {
-    if (!a.kept_cnt || (a.Hm != a.Hk && a.Hm != a.Hq) || a.nb_w <= 0 || a.nb_q < (a.max_q + 126) / 64)
+    if (!a.kept_cnt || (a.Hm != a.Hk && a.Hm != a.Hq) || a.nb_w <= 0 || a.nb_q < ((int64_t)a.max_q + 126) / 64)
       return TASFT_ERR_INVALID_ARG;
   }
   if (a.T == 0) return TASFT_OK;

@@ -297,7 +297,7 @@ extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_s
       a.num_pages <= 0 || a.page_size <= 0)
     return TASFT_ERR_INVALID_ARG;
   if (!a.cu_seqlens || !a.kv_len || !a.block_table || !a.k_pages || !a.v_pages) return TASFT_ERR_INVALID_ARG;
-  if (a.NBq < (a.max_q + 126) / 64 || a.NBq > 65535) return TASFT_ERR_INVALID_ARG;
+  if (a.NBq < ((int64_t)a.max_q + 126) / 64 || a.NBq > 65535) return TASFT_ERR_INVALID_ARG;
   if (a.pooled_k && a.NBk <= 0) return TASFT_ERR_INVALID_ARG;
   if (a.rot < 0 || a.rot > a.D || (a.rot > 0 && !a.inv_freq)) return TASFT_ERR_INVALID_ARG;
   if (a.k_stride[3] != 1 || a.v_stride[3] != 1) return TASFT_ERR_INVALID_ARG;

@@ -139,3 +139,11 @@ def test_frequencies():
             T.rope_inv_freq(64, 10000.0, bad)
     with pytest.raises(T.ValidationError):
         T.rope_inv_freq(63)
+
+
+@pytest.mark.parametrize("max_q", [2**31 - 126, 2**31 - 1])
+def test_rows_for_the_largest_counts_do_not_wrap(max_q):
+    """Too few rows for so many new tokens, although max_q + 126 leaves 32 bits."""
+    lists = dict(kept_idx=4096, kept_cnt=4096, Hm=2, nb_q=2, nb_w=4)
+    assert L.lib().tasft_bsa_chunk_paged_fwd(C.byref(chunk_args(max_q=max_q, **lists)), None) == -1
+    assert L.lib().tasft_rope_append_paged(C.byref(rope_args(max_q=max_q)), None) == -1
