@@ -6,6 +6,7 @@ fallback: if the shared object is missing or fails to load, every op raises.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 import struct
 from pathlib import Path
@@ -312,7 +313,22 @@ def packed(cls):
     fmt = "".join(f"{t._length_}{codes[t._type_]}" if hasattr(t, "_length_") else codes[t] for _, t in cls._fields_)
     pack = struct.Struct("@" + fmt)
     assert pack.size <= C.sizeof(cls) < pack.size + 8  # the tail padding is the struct's own
-    return pack.pack if pack.size == C.sizeof(cls) else struct.Struct(f"@{fmt}{C.sizeof(cls) - pack.size}x").pack
+    pack = (pack if pack.size == C.sizeof(cls) else struct.Struct(f"@{fmt}{C.sizeof(cls) - pack.size}x")).pack
+
+    kinds = [t._type_ if hasattr(t, "_length_") else t for _, t in cls._fields_ for _ in range(getattr(t, "_length_", 1))]
+    floats = [i for i, t in enumerate(kinds) if t is C.c_float]
+    most = torch.finfo(torch.float32).max
+
+    def args(*values) -> bytes:
+        try:
+            for i in floats:  # struct makes them infinite
+                if most < abs(values[i]) < math.inf:
+                    raise OverflowError(f"{values[i]} is out of range in 32 bits")
+            return pack(*values)
+        except (struct.error, OverflowError) as e:
+            raise KernelError(f"{cls.__name__}: {e}", context={"values": list(values)}) from e
+
+    return args
 
 
 def launch(fn, args, gpu: int) -> int:

@@ -44,6 +44,8 @@
 #include "chunk.cuh"
 #include "tc.cuh"
 
+#include <cfloat>
+
 namespace tasft {
 
 namespace {
@@ -1362,7 +1364,7 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   if (a.Hk == 1) a.k_stride[2] = a.v_stride[2] = a.D;
   if (a.num_pages == 1) a.k_stride[0] = a.v_stride[0] = a.D;
   if (a.B <= 0 || a.T < 0 || a.Hq <= 0 || a.Hk <= 0 || a.D <= 0 || a.Hq % a.Hk != 0 || a.max_q <= 0 ||
-      a.max_pages <= 0 || a.num_pages <= 0 || !(a.scale > 0.f))
+      a.max_pages <= 0 || a.num_pages <= 0 || !(a.scale > 0.f && a.scale <= FLT_MAX))
     return TASFT_ERR_INVALID_ARG;
   if (!a.cu_seqlens || !a.kv_len || !a.block_table || !a.k_pages || !a.v_pages) return TASFT_ERR_INVALID_ARG;
   if (a.k_stride[3] != 1 || a.v_stride[3] != 1) return TASFT_ERR_INVALID_ARG;

@@ -147,3 +147,16 @@ def test_rows_for_the_largest_counts_do_not_wrap(max_q):
     lists = dict(kept_idx=4096, kept_cnt=4096, Hm=2, nb_q=2, nb_w=4)
     assert L.lib().tasft_bsa_chunk_paged_fwd(C.byref(chunk_args(max_q=max_q, **lists)), None) == -1
     assert L.lib().tasft_rope_append_paged(C.byref(rope_args(max_q=max_q)), None) == -1
+
+
+@pytest.mark.parametrize("fields", [dict(max_q=2**31), dict(B=-(2**31) - 1), dict(scale=1e300)])
+def test_numbers_that_do_not_fit_their_field_are_refused(fields):
+    values = []
+    for name, kind in L.ChunkArgs._fields_:
+        values += [fields.get(name, 0)] * getattr(kind, "_length_", 1)
+    with pytest.raises(T.KernelError):
+        L.packed(L.ChunkArgs)(*values)
+
+
+def test_an_infinite_scale_is_refused():
+    assert L.lib().tasft_bsa_chunk_paged_fwd(C.byref(chunk_args(scale=math.inf)), None) == -1
