@@ -301,7 +301,7 @@ def bsa_chunk_paged(
     q ``[T, Hq, D]``, pages ``[num_pages, page_size, Hk, D]`` with the new keys and values already
     in them (:func:`rope_append_paged`), ``kept`` lists ``[B, Hk or Hq, NBq, W]`` with at least
     ``chunk_rows(max_new)`` rows, ascending. ``scale`` defaults to ``1 / sqrt(D)``. Returns
-    ``[T, Hq, D]`` (``out``; rows outside all sequences stay as they were, undefined in a new
+    ``[T, Hq, D]`` (``out``, which may be q itself; rows outside all sequences stay as they were, undefined in a new
     tensor); a token with nothing kept gets 0. ``err``: optional int32 error word, see ``include/tasft_b200.h``. bf16 / f16, D 64
     or 128, page size 16, 32, 64 or 128. What the cache holds from ``kv_len`` on, behind a
     token's own position or in blocks its list does not keep never reaches its row, infinities

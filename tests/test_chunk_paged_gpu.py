@@ -310,3 +310,17 @@ def test_graph_replay_follows_its_inputs():
     torch.cuda.synchronize()
     o, a = R.attend(q, kp, vp, table, [2, 31, 2], [398, 0, 28])
     assert ((out.double() - o).abs() <= R.attend_bound(o, a, torch.bfloat16, 600)).all()
+
+
+@pytest.mark.parametrize("lists", [None, "kv", "q"])
+@pytest.mark.parametrize("new,ctx", [([1, 90, 300], [4000, 0, 700]), ([1], [6000]), ([513], [5000])])
+def test_out_may_be_q(lists, new, ctx):
+    """Each tile reads its own rows of q before it writes them, tiles in pieces are written last."""
+    q, kp, vp, table, cu, kv_len, g = case(new, ctx, 8, 2, 128, 16, torch.bfloat16, seed=21)
+    kept = None
+    if lists is not None:
+        width = max((n + c + 63) // 64 for n, c in zip(new, ctx))
+        kept = T.KeptBlocks(*R.random_lists(new, ctx, 2 if lists == "kv" else 8, width, DEV, g, 0.5, True, 0.0))
+    want = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, max(new), kept)
+    got = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, max(new), kept, out=q)
+    assert got is q and torch.equal(got, want)
