@@ -263,8 +263,9 @@ template <typename T, bool kMixed>
 int run(const tasft_rope_append_args& a, cudaStream_t st) {
   auto kern = rope_append_kernel<T, kMixed>;
   const int smem = kRopeRows * a.rot * (int)sizeof(float);  // cos and sin, rot / 2 each
+  constexpr int kPlaces = 2 * kRopeBlk * (int)sizeof(int64_t);  // static, and counted against the limit too
   static std::atomic<uint64_t> allowed{0};
-  if (smem > 48 * 1024 && !allow_smem(kern, kRopeRows * 256 * (int)sizeof(float), allowed)) return TASFT_ERR_CUDA;
+  if (smem + kPlaces > 48 * 1024 && !allow_smem(kern, kRopeRows * 256 * (int)sizeof(float), allowed)) return TASFT_ERR_CUDA;
   const int z = (a.Hq + 2 * a.Hk + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
   if (a.B > 65535) return TASFT_ERR_TOO_LARGE;
   kern<<<dim3((unsigned)z, (unsigned)a.NBq, (unsigned)a.B), kRopeThreads, smem, st>>>(a);

@@ -1,0 +1,38 @@
+"""Edges of the rotary append into a paged cache."""
+from __future__ import annotations
+
+import os
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
+
+# the first call of a process, which no earlier one has given a larger limit
+WIDE = """
+import sys
+import torch
+import tasft_b200 as T
+rot, dtype, mixed = int(sys.argv[1]), getattr(torch, sys.argv[2]), sys.argv[3] == "mixed"
+x = torch.ones(3, 4, 256, device="cuda").to(dtype)
+kp, vp = (torch.zeros(1, 16, 1, 256, device="cuda", dtype=dtype) for _ in range(2))
+ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+freq, _ = T.rope_inv_freq(rot, device="cuda")
+out, _ = T.rope_append_paged(x[:, :2], x[:, 2:3], x[:, 3:], freq, kp, vp, ints(0).view(1, 1), ints(0, 3), ints(3), 3,
+                             interleaved=mixed)
+torch.cuda.synchronize()
+assert torch.equal(out[0], x[0, :2]) and torch.equal(vp[0, :3, 0], x[:, 3]) and (out[1] != x[1, :2]).any()
+"""
+
+
+@pytest.mark.parametrize("rot", [176, 192, 208])
+@pytest.mark.parametrize("dtype,mixed", [("bfloat16", "half"), ("float16", "mixed"), ("float32", "half")])
+def test_first_call_of_a_process_at_wide_rotations(rot, dtype, mixed):
+    """64 rows of cos and sin and the kernel's own tables pass 48 KB from rot = 192 on."""
+    env = dict(os.environ, PYTHONPATH=str(ROOT))
+    got = subprocess.run([sys.executable, "-c", WIDE, str(rot), dtype, mixed], env=env, capture_output=True, text=True,
+                         timeout=300)
+    assert got.returncode == 0, got.stderr[-2000:]
