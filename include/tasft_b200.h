@@ -67,7 +67,7 @@ extern "C" {
 #define TASFT_ERR_INVALID_ARG    -1  /* null pointer, bad shape, bad stride */
 #define TASFT_ERR_UNSUPPORTED    -2  /* dtype / head_dim / block size not built */
 #define TASFT_ERR_CUDA           -3  /* a CUDA runtime call failed */
-#define TASFT_ERR_WORKSPACE      -4  /* workspace missing or too small */
+#define TASFT_ERR_WORKSPACE      -4  /* workspace missing, too small or misaligned */
 #define TASFT_ERR_TOO_LARGE      -5  /* a size exceeds a fixed capacity */
 
 /* device error word bits (OR-ed into *err when err != NULL) */
@@ -396,7 +396,7 @@ typedef struct {
   int32_t Hm;               /* heads of the lists: Hk (one list per group) or Hq */
   int32_t nb_q, nb_w;       /* rows per head, at least (max_q + 126) / 64; entries per row */
   float scale;              /* softmax scale, > 0 */
-  void* workspace;          /* tasft_chunk_workspace_size() bytes */
+  void* workspace;          /* tasft_chunk_workspace_size() bytes on a 32-byte boundary (TASFT_ERR_WORKSPACE) */
   int64_t workspace_bytes;
   int32_t* err;
 } tasft_chunk_args;

@@ -22,7 +22,7 @@ STATUS = {
     -1: "invalid argument",
     -2: "unsupported dtype, head_dim or block size",
     -3: "CUDA runtime error",
-    -4: "workspace missing or too small",
+    -4: "workspace missing, too small or misaligned",
     -5: "size exceeds a fixed capacity",
 }
 DEVERR_INDEX, DEVERR_TIMEOUT, DEVERR_ORDER = 1, 2, 4

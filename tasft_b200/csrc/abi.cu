@@ -71,7 +71,7 @@ extern "C" const char* tasft_status_string(int status) {
     case TASFT_ERR_INVALID_ARG: return "invalid argument";
     case TASFT_ERR_UNSUPPORTED: return "unsupported dtype, head_dim or block size";
     case TASFT_ERR_CUDA: return "CUDA runtime error";
-    case TASFT_ERR_WORKSPACE: return "workspace missing or too small";
+    case TASFT_ERR_WORKSPACE: return "workspace missing, too small or misaligned";
     case TASFT_ERR_TOO_LARGE: return "size exceeds a fixed capacity";
     default: return "unknown status";
   }

@@ -1397,6 +1397,7 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   sh.may_cut = sh.mode == 0 ? bound > kChunkMergeCost
                             : ((tiles + G - 1) / G * G - tiles) * bound > kChunkMergeCost * G;
   if (!a.workspace || a.workspace_bytes < ws_layout(sh, a.D, (int)G).bytes) return TASFT_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(a.workspace) & 31u) != 0) return TASFT_ERR_WORKSPACE;  // 32-byte stores of partials
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   const bool f16 = a.dtype == TASFT_F16;
