@@ -158,8 +158,9 @@ TASFT_API int tasft_qkv_rope_pool(const tasft_qkv_args* args, tasft_stream_t str
  * (tasft/modules/tasft_attention.py:872-908 takes cos and sin as given).
  * q_out may be q. f32 / bf16 / f16; D and rot multiples of two 16-byte vectors (16 columns, 8 in
  * f32), D <= 256; rows on 16-byte boundaries. TASFT_DEVERR_INDEX: a page out of range (its
- * rows are not written) or a sequence whose lengths do not fit T, max_q, each other or the
- * table (left out). A page must not be written through two sequences in one call. */
+ * rows are not written), a key block from NBk on (its mean has no place; its rows are written)
+ * or a sequence whose lengths do not fit T, max_q, each other or the table (left out). A page
+ * must not be written through two sequences in one call. */
 typedef struct {
   const void* q;            /* [T, Hq, D] */
   const void* k;            /* [T, Hk, D] */

@@ -157,10 +157,10 @@ def rope_append_paged(
     ``[rot / 2]`` fp64 or fp32 as :func:`rope_inv_freq` gives it: the first ``rot`` columns of a head
     turn, in pairs ``(i, i + rot/2)`` or, ``interleaved``, ``(2i, 2i + 1)``; cos and sin are multiplied
     by ``attention_scaling``. ``max_new``: most new tokens of a sequence. With ``pooled_k`` (fp32
-    ``[B, Hk, NBk, D]``, updated in place: the mean of every key block that got new tokens) also
-    computes the means of the new queries. Returns ``(q, pooled_q)``: rotated q (``out``, which may
-    be q itself; rows outside all sequences are not written) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for
-    :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
+    ``[B, Hk, NBk, D]``, updated in place: the mean of every key block that got new tokens; one from
+    NBk on is left out and reported in ``err``) also computes the means of the new queries. Returns
+    ``(q, pooled_q)``: rotated q (``out``, which may be q itself; rows outside all sequences are not
+    written) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
     256. The packed, paged counterpart of :func:`qkv_rope_pool`, which takes cos and sin as tables."""
     name = "rope_append_paged"
     gpu, qs, ks = q.get_device(), q.shape, k_pages.shape

@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasf
       for (int d = lane; d < a.D; d += 32) a.pooled_q[(((int64_t)b * a.Hq + h) * a.NBq + qi) * a.D + d] = 0.f;
     return;
   }
+  if (a.pooled_k && blk >= a.NBk && blockIdx.x == 0 && threadIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
   const int p0 = blk * kRopeBlk;
   const int r_lo = max(ctx - p0, 0), r_hi = min(len - p0, kRopeBlk);  // rows of the block with new tokens
 

@@ -7,8 +7,13 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
+
+import paged_oracle as R
+import tasft_b200 as T
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda"
 ROOT = Path(__file__).resolve().parent.parent
 
 # the first call of a process, which no earlier one has given a larger limit
@@ -36,3 +41,28 @@ def test_first_call_of_a_process_at_wide_rotations(rot, dtype, mixed):
     got = subprocess.run([sys.executable, "-c", WIDE, str(rot), dtype, mixed], env=env, capture_output=True, text=True,
                          timeout=300)
     assert got.returncode == 0, got.stderr[-2000:]
+
+
+def batch(new, ctx, Hq, Hk, D, page, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    kp, vp, table, cu, kv_len = R.layout(new, ctx, page, Hk, D, dtype, DEV, g)
+    rows = torch.randn(sum(new), Hq + 2 * Hk, D, generator=g, device=DEV).to(dtype)
+    freq, _ = T.rope_inv_freq(D, device=DEV)
+    return rows[:, :Hq], rows[:, Hq:Hq + Hk], rows[:, Hq + Hk:], freq, kp, vp, table, cu, kv_len
+
+
+def test_means_that_have_no_place_are_reported():
+    """A third block of a sequence, and room for the means of two: nothing is written beside them."""
+    for n, nbk, bit in ((100, 2, 0), (101, 2, 1), (101, 3, 0), (1, 1, 1)):
+        args = batch([n], [28], 4, 2, 64, 16, torch.bfloat16)
+        if n == 1:
+            args = batch([n], [64], 4, 2, 64, 16, torch.bfloat16)
+        space = torch.full((3, 2, nbk, 64), 5.0, device=DEV)
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        T.rope_append_paged(*args, n, pooled_k=space[1:2], err=err)
+        assert int(err.item()) == bit, (n, nbk)
+        assert (space[0] == 5).all() and (space[2] == 5).all()
+        # without means there is nothing to report
+        err.zero_()
+        T.rope_append_paged(*args, n, err=err)
+        assert int(err.item()) == 0
