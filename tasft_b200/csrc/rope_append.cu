@@ -230,9 +230,9 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasf
           turn<T, kMixed>(u1[i], u2[i], reinterpret_cast<const float*>(cs),
                           reinterpret_cast<const float*>(cs + kQuads / 2));
         }
-        if (sum) add_pair<T>(acc, u1[i], u2[i]);
         const int64_t off = is_q ? r * a.o_stride[0] : at[r];
-        if (!is_q && off < 0) continue;  // its page is not there
+        if (!is_q && off < 0) continue;  // its page is not there: it is not held, and in no mean
+        if (sum) add_pair<T>(acc, u1[i], u2[i]);
         *reinterpret_cast<uint4*>(out + off + c1) = u1[i];
         *reinterpret_cast<uint4*>(out + off + c2) = u2[i];
       }

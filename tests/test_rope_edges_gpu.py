@@ -66,3 +66,22 @@ def test_means_that_have_no_place_are_reported():
         err.zero_()
         T.rope_append_paged(*args, n, err=err)
         assert int(err.item()) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_without_a_page_take_no_part_in_a_mean(dtype):
+    """A key mean is that of what the cache holds: new rows whose page is not there are not in it, as
+    earlier ones are not."""
+    q, k, v, freq, kp, vp, table, cu, kv_len = batch([40], [24], 4, 2, 64, 16, dtype, seed=1)
+    for gone in (0, 2, 3):  # rows 0 to 15 came earlier, 32 to 47 and 48 to 63 are new
+        t = table.clone()
+        t[0, gone] = -1 if gone == 2 else kp.shape[0]
+        k1, means = kp.clone(), torch.zeros(1, 2, 1, 64, device=DEV)
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        T.rope_append_paged(q, k, v, freq, k1, vp.clone(), t, cu, kv_len, 40, pooled_k=means, err=err)
+        assert int(err.item()) & 1
+        held = R.cached(k1, table[0], 64).double()
+        held[16 * gone:16 * gone + 16] = 0
+        # 63 fp32 additions, each at most half a step off
+        tol = 64 * 2.0 ** -24 * held.abs().sum(0) / 64
+        assert ((means[0, :, 0].double() - held.sum(0) / 64).abs() <= tol).all()
