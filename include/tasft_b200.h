@@ -375,8 +375,8 @@ TASFT_API int tasft_bsa_decode_paged_fwd(const tasft_paged_decode_args* args, ta
  * bf16 / f16, D 64 or 128, block 64, page_size 16, 32, 64 or 128, Hq / Hk <= 64; pointers and
  * strides of whole 16 bytes. Reported in *err without a fault: TASFT_DEVERR_INDEX (a page or
  * kept block out of range: skipped; a sequence whose lengths do not fit T, max_q, each other
- * or the table: its rows are left out), TASFT_DEVERR_ORDER (a list that does not ascend: the
- * entry is skipped). Cache rows from kv_len on, and
+ * or the table: its rows are left out), TASFT_DEVERR_ORDER (a list that does not ascend: an
+ * entry not above all those before it is skipped). Cache rows from kv_len on, and
  * values of K and V that are not finite behind a token's mask, never reach its row. */
 typedef struct {
   const void* q;            /* [T, Hq, D] */

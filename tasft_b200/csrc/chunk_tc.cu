@@ -105,6 +105,33 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
+// Up to 32 consecutive entries of a kept list, one a lane (INT32_MAX behind its end): whether the
+// lane's stands above every entry before it, `top` being the largest of those before lane 0's, and
+// whether it is an index at all. `top` moves on to the largest of the first n. Entries that ascend,
+// as they should, take one comparison; the running maximum is for those that do not.
+struct ListCheck {
+  bool index, order;
+};
+__device__ __forceinline__ ListCheck check_entries(int kb, int n, int lane, int& top) {
+  int before = __shfl_up_sync(0xffffffffu, kb, 1);
+  if (lane == 0) before = top;
+  const bool in = lane < n;
+  if (__any_sync(0xffffffffu, in && (kb < 0 || kb <= before))) {
+    int upto = in ? kb : -1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto = max(upto, x);
+    }
+    before = __shfl_up_sync(0xffffffffu, upto, 1);
+    before = lane == 0 ? top : max(before, top);
+    top = max(top, __shfl_sync(0xffffffffu, upto, 31));
+  } else if (n > 0) {
+    top = __shfl_sync(0xffffffffu, kb, n - 1);
+  }
+  return {in && kb >= 0, in && kb > before};
+}
+
 // One list segment and the tile it belongs to.
 struct Work {
   int n;            // entries; -1: no more work
@@ -557,8 +584,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       // ---- the piece's segments ----
       int at = lo;                       // next list position or block
       int pt[2] = {0, 0};                // mode 2: next position of each list
-      int prev[2] = {-1, -1};            // last accepted block of each list
-      if (!done && sh.mode == 1 && lo > 0) prev[0] = idx[0][lo - 1];
+      int top[2] = {-1, -1};             // largest entry so far of each list
+      if (!done && sh.mode == 1 && lo > 0) {  // of the pieces before this one
+        for (int i = lane; i < lo; i += 32) top[0] = max(top[0], idx[0][i]);
+        top[0] = __reduce_max_sync(0xffffffffu, top[0]);
+      }
       bool first = true;
       while (ok) {
         const int lb = u & 1;
@@ -587,18 +617,16 @@ __global__ void __launch_bounds__(kThreads, 2)
             while (pt[x] < cnt[x]) {
               const int i = pt[x] + lane;
               const int kb = i < cnt[x] ? idx[x][i] : INT32_MAX;
-              int before = __shfl_up_sync(0xffffffffu, kb, 1);
-              if (lane == 0) before = prev[x];
               const bool mine = kb < wend;  // this window's (a list ascends, so a prefix)
               const unsigned out = __ballot_sync(0xffffffffu, !mine);
               const int take = out ? __ffs(out) - 1 : 32;
+              const ListCheck good = check_entries(kb, take, lane, top[x]);
               if (lane < take) {
-                if (kb < 0) set_err(a.err, TASFT_DEVERR_INDEX);
-                else if (kb <= before) set_err(a.err, TASFT_DEVERR_ORDER);
+                if (!good.index) set_err(a.err, TASFT_DEVERR_INDEX);
+                else if (!good.order) set_err(a.err, TASFT_DEVERR_ORDER);
                 else if (kb >= at && kb <= qb[x])
                   atomicOr(&bitmap[x * (kSeg / 32) + ((kb - at) >> 5)], 1u << ((kb - at) & 31));
               }
-              if (take > 0) prev[x] = __shfl_sync(0xffffffffu, kb, take - 1);
               pt[x] += take;
               if (take < 32) break;
             }
@@ -622,17 +650,10 @@ __global__ void __launch_bounds__(kThreads, 2)
             bool good = i < end;
             if (sh.mode == 1) {
               kb = good ? idx[0][i] : INT32_MAX;
-              int before = __shfl_up_sync(0xffffffffu, kb, 1);
-              if (lane == 0) before = prev[0];
-              prev[0] = __shfl_sync(0xffffffffu, kb, min(31, end - 1 - i0));
-              if (good && kb < 0) {
-                set_err(a.err, TASFT_DEVERR_INDEX);
-                good = false;
-              } else if (good && kb <= before) {
-                set_err(a.err, TASFT_DEVERR_ORDER);
-                good = false;
-              }
-              if (kb > qb[0]) good = false;
+              const ListCheck c = check_entries(kb, min(32, end - i0), lane, top[0]);
+              if (good && !c.index) set_err(a.err, TASFT_DEVERR_INDEX);
+              else if (good && !c.order) set_err(a.err, TASFT_DEVERR_ORDER);
+              good = c.index && c.order && kb <= qb[0];
             }
             const unsigned bal = __ballot_sync(0xffffffffu, good);
             if (good) list[n + __popc(bal & ((1u << lane) - 1u))] = kb | (1 << (kKbBits + 4));
