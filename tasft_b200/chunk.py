@@ -47,9 +47,13 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: dict | None =
       original context and ``b = clip((t_i - low_freq_factor) / (high_freq_factor -
       low_freq_factor), 0, 1)``: ``f_i (b + (1 - b) / factor)``;
     * ``yarn``: with ``d(t) = rotary_dim * ln(original / (2pi t)) / (2 ln base)``, ``lo =
-      max(floor(d(beta_fast)), 0)``, ``hi = min(ceil(d(beta_slow)), rotary_dim - 1)`` and ``r =
-      clip((i - lo) / (hi - lo), 0, 1)``: ``f_i ((1 - r) + r / factor)``; cos and sin are scaled by
-      ``attention_factor``, ``0.1 ln(factor) + 1`` unless given.
+      max(floor(d(beta_fast)), 0)``, ``hi = min(ceil(d(beta_slow)), rotary_dim - 1)`` (neither rounded
+      where ``truncate`` is false) and ``r = clip((i - lo) / (hi - lo), 0, 1)``: ``f_i ((1 - r) + r /
+      factor)``. Cos and sin are scaled by ``attention_factor`` where given; with ``m(c) = 0.1 c
+      ln(factor) + 1``, by ``m(mscale) / m(mscale_all_dim)`` where both are, else by ``m(1)``. (What
+      such a model multiplies its softmax scale with is the caller's, as ``scale`` of
+      :func:`bsa_chunk_paged`.) One of the two alone, where that is not ``m(1)`` either way of reading
+      it, is refused.
     """
     if rotary_dim <= 0 or rotary_dim % 2 or base <= 0:
         raise ValidationError("rotary_dim must be even and positive, base positive",
@@ -86,15 +90,33 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: dict | None =
             def dim_of(t: float) -> float:
                 return rotary_dim * math.log(original / (2 * math.pi * t)) / (2 * math.log(base))
 
-            lo = max(math.floor(dim_of(float(scaling.get("beta_fast") or 32.0))), 0)
-            hi = min(math.ceil(dim_of(float(scaling.get("beta_slow") or 1.0))), rotary_dim - 1)
+            lo, hi = dim_of(float(scaling.get("beta_fast") or 32.0)), dim_of(float(scaling.get("beta_slow") or 1.0))
+            if scaling.get("truncate") is None or scaling["truncate"]:
+                lo, hi = math.floor(lo), math.ceil(hi)
+            lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
             ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
             f = f * ((1 - ramp) + ramp / factor)
-            given = scaling.get("attention_factor")
-            attention = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+            attention = _yarn_attention(scaling, factor)
     else:
         raise ValidationError(f"unknown rope scaling '{kind}'", context={"scaling": dict(scaling)})
     return (f if device is None else f.to(device)), attention
+
+
+def _yarn_attention(scaling: dict, factor: float) -> float:
+    """The factor on cos and sin of ``yarn``."""
+    given, part, whole = (scaling.get(n) for n in ("attention_factor", "mscale", "mscale_all_dim"))
+
+    def m(c: float) -> float:
+        return 0.1 * c * math.log(factor) + 1.0
+
+    if given is not None:
+        return float(given)
+    if part and whole:
+        return m(float(part)) / m(float(whole))
+    if whole or part not in (None, 1):
+        raise ValidationError("yarn needs mscale and mscale_all_dim together (or attention_factor)",
+                              context={"scaling": dict(scaling)})
+    return m(1.0)
 
 
 _rope_args = L.packed(L.RopeAppendArgs)

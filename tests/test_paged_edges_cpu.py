@@ -2,9 +2,12 @@
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import pytest
+import torch
 
+import tasft_b200 as T
 from tasft_b200 import _lib as L
 
 
@@ -23,3 +26,45 @@ def chunk_args(**kw):
 def test_a_workspace_off_32_byte_boundaries_is_refused(at):
     """Partial results are stored 32 bytes at a time."""
     assert L.lib().tasft_bsa_chunk_paged_fwd(C.byref(chunk_args(workspace=at)), None) == -4
+
+
+def yarn(i, dim, base, factor, original, fast=32.0, slow=1.0, truncate=True):
+    """Frequency i from the definition: pairs that turn more than ``fast`` times within the original
+    context stay, those that turn less than ``slow`` times are divided, a ramp over i between."""
+    def place(turns):  # the i (not whole) whose pair turns so often
+        return dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+    lo, hi = place(fast), place(slow)
+    if truncate:
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, dim - 1)
+    part = min(1.0, max(0.0, (i - lo) / (hi - lo)))
+    f = base ** (-2 * i / dim)
+    return f * (1 - part) + f / factor * part
+
+
+@pytest.mark.parametrize("dim,base,factor,original", [(64, 150000.0, 32.0, 4096), (128, 1e6, 4.0, 32768),
+                                                      (64, 10000.0, 40.0, 4096)])
+@pytest.mark.parametrize("extra", [{}, {"truncate": True}, {"truncate": False}, {"beta_fast": 16.0, "truncate": False},
+                                   {"beta_slow": 2.0}])
+def test_yarn_frequencies_with_their_options(dim, base, factor, original, extra):
+    f, a = T.rope_inv_freq(dim, base, dict(rope_type="yarn", factor=factor, original_max_position_embeddings=original,
+                                           **extra))
+    want = [yarn(i, dim, base, factor, original, extra.get("beta_fast", 32.0), extra.get("beta_slow", 1.0),
+                 extra.get("truncate", True)) for i in range(dim // 2)]
+    assert torch.allclose(f, torch.tensor(want, dtype=torch.float64), rtol=1e-12, atol=0)
+    assert a == pytest.approx(0.1 * math.log(factor) + 1, rel=1e-15)
+
+
+def test_yarn_factor_on_cos_and_sin():
+    s = dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096)
+    m = lambda c: 0.1 * c * math.log(40.0) + 1  # noqa: E731
+    for extra, want in (({}, m(1)), ({"mscale": 1.0, "mscale_all_dim": 1.0}, 1.0),
+                        ({"mscale": 0.707, "mscale_all_dim": 1.0}, m(0.707) / m(1)), ({"mscale": 1.0}, m(1)),
+                        ({"mscale": 1.0, "mscale_all_dim": 0.0}, m(1)), ({"mscale": None, "mscale_all_dim": None}, m(1)),
+                        ({"mscale": 1.0, "mscale_all_dim": 2.0, "attention_factor": 1.25}, 1.25)):
+        assert T.rope_inv_freq(64, 10000.0, dict(s, **extra))[1] == pytest.approx(want, rel=1e-15), extra
+    assert T.rope_inv_freq(64, 10000.0, dict(s, factor=1.0, mscale=1.0, mscale_all_dim=0.5))[1] == 1.0
+    # one of the two alone means different things to different models
+    for extra in ({"mscale": 0.707}, {"mscale_all_dim": 1.0}, {"mscale": 0.707, "mscale_all_dim": 0.0}):
+        with pytest.raises(T.ValidationError):
+            T.rope_inv_freq(64, 10000.0, dict(s, **extra))
