@@ -54,14 +54,21 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: dict | None =
       such a model multiplies its softmax scale with is the caller's, as ``scale`` of
       :func:`bsa_chunk_paged`.) One of the two alone, where that is not ``m(1)`` either way of reading
       it, is refused.
+
+    Options of the other kinds are passed over, as is one that is None. Any other option would change
+    the result and is refused, a ``rope_theta`` that is not ``base`` among them.
     """
-    if rotary_dim <= 0 or rotary_dim % 2 or base <= 0:
+    if rotary_dim <= 0 or rotary_dim % 2 or not 0.0 < base < math.inf:
         raise ValidationError("rotary_dim must be even and positive, base positive",
                               context={"rotary_dim": rotary_dim, "base": base})
     i = torch.arange(rotary_dim // 2, dtype=torch.float64)
     f = float(base) ** (-2.0 * i / rotary_dim)
     scaling = scaling or {}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    strange = [n for n, x in scaling.items() if n not in _SCALING and x is not None]
+    if strange or scaling.get("rope_theta") not in (None, base):
+        raise ValidationError(f"rope scaling '{kind}': {', '.join(strange) or 'rope_theta'} would change the result",
+                              context={"scaling": dict(scaling), "base": base})
     attention = 1.0
     if kind == "default":
         pass
@@ -70,27 +77,31 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: dict | None =
                 "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
                 "yarn": ("factor", "original_max_position_embeddings")}[kind]
         missing = [n for n in need if scaling.get(n) is None]
-        if missing or not float(scaling["factor"]) >= 1.0:
+        if missing or not _number(scaling, "factor") >= 1.0:
             raise ValidationError(f"rope scaling '{kind}' needs {', '.join(need)}, factor at least 1",
                                   context={"scaling": dict(scaling)})
-        factor = float(scaling["factor"])
+        factor = _number(scaling, "factor")
         if kind == "linear":
             f = f / factor
         elif kind == "llama3":
-            low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+            low, high = _number(scaling, "low_freq_factor"), _number(scaling, "high_freq_factor")
             if not high > low:
                 raise ValidationError("high_freq_factor must be above low_freq_factor",
                                       context={"scaling": dict(scaling)})
-            turns = float(scaling["original_max_position_embeddings"]) * f / (2 * math.pi)
+            turns = _number(scaling, "original_max_position_embeddings") * f / (2 * math.pi)
             blend = ((turns - low) / (high - low)).clamp(0.0, 1.0)
             f = f * (blend + (1 - blend) / factor)
         else:
-            original = float(scaling["original_max_position_embeddings"])
+            original = _number(scaling, "original_max_position_embeddings")
+            fast, slow = (_number(scaling, n) if scaling.get(n) else x for n, x in (("beta_fast", 32.0), ("beta_slow", 1.0)))
+            if not (original > 0 and fast > 0 and slow > 0 and base > 1):
+                raise ValidationError("yarn needs a base above 1, original length and betas above 0",
+                                      context={"scaling": dict(scaling), "base": base})
 
             def dim_of(t: float) -> float:
                 return rotary_dim * math.log(original / (2 * math.pi * t)) / (2 * math.log(base))
 
-            lo, hi = dim_of(float(scaling.get("beta_fast") or 32.0)), dim_of(float(scaling.get("beta_slow") or 1.0))
+            lo, hi = dim_of(fast), dim_of(slow)
             if scaling.get("truncate") is None or scaling["truncate"]:
                 lo, hi = math.floor(lo), math.ceil(hi)
             lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
@@ -102,18 +113,39 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: dict | None =
     return (f if device is None else f.to(device)), attention
 
 
+# what a scaling dictionary may hold; a kind takes no notice of the other kinds' options
+_SCALING = frozenset((
+    "rope_type", "type", "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor",
+    "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate",
+    "rope_theta",             # the base: as the call's
+    "partial_rotary_factor",  # in rotary_dim already
+    "finetuned",              # how the weights came about
+))
+
+
+def _number(scaling: dict, name: str) -> float:
+    try:
+        x = float(scaling[name])
+    except (TypeError, ValueError):
+        x = math.nan
+    if not math.isfinite(x):
+        raise ValidationError(f"rope scaling: {name} must be a finite number", context={"scaling": dict(scaling)})
+    return x
+
+
 def _yarn_attention(scaling: dict, factor: float) -> float:
     """The factor on cos and sin of ``yarn``."""
-    given, part, whole = (scaling.get(n) for n in ("attention_factor", "mscale", "mscale_all_dim"))
+    given, part, whole = (_number(scaling, n) if scaling.get(n) is not None else None
+                          for n in ("attention_factor", "mscale", "mscale_all_dim"))
 
     def m(c: float) -> float:
         return 0.1 * c * math.log(factor) + 1.0
 
     if given is not None:
-        return float(given)
-    if part and whole:
-        return m(float(part)) / m(float(whole))
-    if whole or part not in (None, 1):
+        return given
+    if part and whole and part > 0 and whole > 0:
+        return m(part) / m(whole)
+    if whole or part not in (None, 1.0):
         raise ValidationError("yarn needs mscale and mscale_all_dim together (or attention_factor)",
                               context={"scaling": dict(scaling)})
     return m(1.0)

@@ -68,3 +68,37 @@ def test_yarn_factor_on_cos_and_sin():
     for extra in ({"mscale": 0.707}, {"mscale_all_dim": 1.0}, {"mscale": 0.707, "mscale_all_dim": 0.0}):
         with pytest.raises(T.ValidationError):
             T.rope_inv_freq(64, 10000.0, dict(s, **extra))
+
+
+LLAMA3 = dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+              original_max_position_embeddings=8192)
+YARN = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768)
+
+
+@pytest.mark.parametrize("scaling", [None, {"rope_type": "linear", "factor": 4.0}, LLAMA3, YARN])
+def test_options_that_would_change_the_result_are_not_dropped(scaling):
+    """An option that nothing here computes is refused; one that says what the call says already, or
+    that belongs to another kind, is not."""
+    s = scaling or {"rope_type": "default"}
+    want = T.rope_inv_freq(64, 5e5, scaling)
+    for extra in ({"rope_theta": 5e5}, {"partial_rotary_factor": 0.5}, {"type": s["rope_type"]}, {"unknown": None},
+                  {"finetuned": True}, {"original_max_position_embeddings": 32768 if s is YARN else 8192}):
+        got = T.rope_inv_freq(64, 5e5, {**s, **extra})
+        assert torch.equal(got[0], want[0]) and got[1] == want[1]
+    for extra in ({"rope_theta": 1e4}, {"mrope_section": [16, 24, 24]}, {"attn_factor": 1.2},
+                  {"long_factor": [1.0] * 32}, {"extrapolation_factor": 0.5}):
+        with pytest.raises(T.ValidationError):
+            T.rope_inv_freq(64, 5e5, {**s, **extra})
+
+
+@pytest.mark.parametrize("args", [
+    (64, math.nan), (64, math.inf), (64, 1.0, YARN), (64, 1e4, {**YARN, "original_max_position_embeddings": 0}),
+    (64, 1e4, {**YARN, "original_max_position_embeddings": -4096}), (64, 1e4, {**YARN, "beta_fast": -1.0}),
+    (64, 1e4, {**YARN, "factor": math.inf}), (64, 1e4, {**YARN, "factor": math.nan}),
+    (64, 1e4, {**YARN, "beta_slow": math.inf}), (64, 1e4, {**LLAMA3, "original_max_position_embeddings": math.inf}),
+    (64, 1e4, {**LLAMA3, "low_freq_factor": math.nan}), (64, 1e4, {**YARN, "attention_factor": math.nan}),
+    (64, 1e4, {**YARN, "factor": "wide"}), (64, 1e4, {**YARN, "mscale": 1.0, "mscale_all_dim": -3.0}),
+])
+def test_numbers_without_a_meaning_are_refused(args):
+    with pytest.raises(T.ValidationError):
+        T.rope_inv_freq(*args)
