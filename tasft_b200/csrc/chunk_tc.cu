@@ -3,7 +3,8 @@
 // For token t at position p of its sequence and query head h of kv-head g,
 //   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q.k_j,  m = max_j s_j,
 // over the kept keys j <= p: one pass over the keys with the running (m, sum, o) of the
-// online softmax in fp32. P is rounded to the value dtype for P.V, as the prefill does.
+// online softmax in fp32. P is rounded to the value dtype for P.V, as the prefill does (bf16: half
+// a step, 2^-8 of each p; fp16: 2^-11 of it or, where it is small, 2^-31 of the largest).
 //
 // Tile = 128 rows that share one kv-head, filled by mode:
 //   0  every block kept: all query heads of a group times as many tokens as fit
@@ -56,6 +57,9 @@ constexpr int kSeg = 128;                  // entries of a list segment
 constexpr uint32_t kTmemCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+// fp16 holds nothing below 2^-25, so many small probabilities beside a large one would come to 0
+// (60000 of 2^-25.4 are 0.14 %): P is held, and l summed, 2^6 times as large, 2^14 at most
+constexpr float kHalfShift = 6.0f;
 
 // entry of a list segment: block index, which of its (up to four) pages are there, slots
 constexpr int kKbBits = 20;
@@ -960,7 +964,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (sv[c] != sv[c]) rs = sv[c];
             }
           } else {
-            const uint64_t sc2 = f2(sl2, sl2), nm2 = f2(-m, -m);
+            const float nm = kF16 ? kHalfShift - m : -m;
+            const uint64_t sc2 = f2(sl2, sl2), nm2 = f2(nm, nm);
             uint64_t rs2 = 0;
 #pragma unroll
             for (int c = 0; c < 32; ++c) {

@@ -1,6 +1,8 @@
 """Edges of the attention of new tokens over a paged cache."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -50,3 +52,29 @@ def test_order_is_kept_across_warps_segments_and_pieces(heads):
         cnt = torch.full((1, 1, 1), len(kept), dtype=torch.int32, device=DEV)
         o, a = R.attend(q, kp, vp, table, [1], [64 * blocks - 1], (idx, cnt))
         assert ((got.double() - o).abs() <= R.attend_bound(o, a, torch.bfloat16, 64 * blocks)).all(), (at, jump)
+
+
+@pytest.mark.parametrize("ctx,D", [(60000, 64), (30000, 128), (9000, 64)])
+@pytest.mark.parametrize("top", [0, 4000])
+def test_many_small_probabilities_in_half_precision(ctx, D, top):
+    """One key far above the others (25.4 in base 2), whose values are 0: the output is the sum of the
+    small ones, each below half the smallest fp16. Held as 2^6 p, a p is off by at most 2^-31 absolute.
+    One tile a CTA, so that tiles stay whole: the same sequence as often as there are SMs."""
+    n, B = ctx + 1, torch.cuda.get_device_properties(0).multi_processor_count
+    g = torch.Generator(device=DEV).manual_seed(3)
+    kp, vp, table, _, _ = R.layout([1], [ctx], 64, 2, D, torch.float16, DEV, g)
+    kp.zero_()
+    vp.copy_(1 + torch.rand(vp.shape, generator=g, device=DEV))
+    page, row = int(table[0, top // 64]), top % 64
+    kp[page, row, :, 0] = 1.0
+    vp[page, row] = 0.0
+    q = torch.zeros(B, 4, D, device=DEV, dtype=torch.float16)
+    q[:, :, 0] = 2.0
+    scale = 25.4 * math.log(2.0) / 2.0
+    out = T.bsa_chunk_paged(q, kp, vp, table.repeat(B, 1), torch.arange(B + 1, dtype=torch.int32, device=DEV),
+                            torch.full((B,), n, dtype=torch.int32, device=DEV), 1, scale=scale)
+    o, a = R.attend(q[:1], kp, vp, table, [1], [ctx], scale=scale)
+    # half a step of the result, 2^-31 for each p (2^6 2^-25.4 is below the normal numbers of fp16)
+    # against a sum of at least 1, and 2^-14 for fp32 scores, exponentials and sums, as in attend_bound
+    bound = 2.0 ** -11 * o.abs() + 2.0 ** -14 * a + n * 2.0 ** -31 * vp.max().item() + 2.0 ** -25
+    assert ((out.double() - o).abs() <= bound).all()
