@@ -21,7 +21,7 @@
  *   tasft_mask_from_scores     soft >= tau (+ tril)       tasft/modules/attn_gate.py:466-477
  *   tasft_qkv_rope_pool        _prepare_qkv head split + rotary + the gate's pooling
  *                              tasft/modules/tasft_attention.py:615-742, attn_gate.py:351-375
- *   tasft_rope_append_paged    (none: the paged, packed form of tasft_qkv_rope_pool)
+ *   tasft_rope_append_paged    (none: the paged, packed form of tasft_qkv_rope_pool); _opt
  *   tasft_select_blocks        (none: top-scored blocks; the reference keeps by threshold)
  *   tasft_bsa_chunk_paged_fwd  (none: the reference's vLLM prefill has no cache behind it,
  *                              tasft/inference/vllm_patch.py:172-196)
@@ -185,6 +185,13 @@ typedef struct {
   int32_t* err;
 } tasft_rope_append_args;
 TASFT_API int tasft_rope_append_paged(const tasft_rope_append_args* args, tasft_stream_t stream);
+
+/* The same with options (0: the call above). TASFT_ROPE_MEAN_NEW: a row of pooled_q is the mean
+ * over the block's new rows, not their sum over the block. A gate that was trained on whole
+ * sequences saw means of full blocks; a single token's sum over 64 is next to nothing to it, and the
+ * rest of the block's queries are gone. */
+#define TASFT_ROPE_MEAN_NEW 1
+TASFT_API int tasft_rope_append_paged_opt(const tasft_rope_append_args* args, int32_t options, tasft_stream_t stream);
 
 /* Kept blocks by score, for the new tokens of a packed batch: row i of sequence b stands for
  * block mine = (kv_len[b] - new) / block + i and keeps blocks [0, first), (mine - local, mine]

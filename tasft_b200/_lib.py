@@ -118,6 +118,9 @@ class PagedDecodeArgs(C.Structure):
 I64x2 = C.c_int64 * 2
 
 
+ROPE_MEAN_NEW = 1  # options of tasft_rope_append_paged_opt
+
+
 class RopeAppendArgs(C.Structure):
     _fields_ = [
         ("q", vp), ("k", vp), ("v", vp), ("q_out", vp), ("k_pages", vp), ("v_pages", vp),
@@ -217,6 +220,7 @@ SIGNATURES = {
     "tasft_mask_from_scores": ([C.POINTER(ThresholdArgs), vp], C.c_int),
     "tasft_qkv_rope_pool": ([C.POINTER(QkvArgs), vp], C.c_int),
     "tasft_rope_append_paged": ([vp, vp], C.c_int),
+    "tasft_rope_append_paged_opt": ([vp, C.c_int32, vp], C.c_int),
     "tasft_select_blocks": ([vp, vp], C.c_int),
     "tasft_chunk_workspace_size": ([C.c_int32] * 7, C.c_int64),
     "tasft_bsa_chunk_paged_fwd": ([vp, vp], C.c_int),
@@ -331,13 +335,13 @@ def packed(cls):
     return args
 
 
-def launch(fn, args, gpu: int) -> int:
+def launch(fn, gpu: int, *args) -> int:
     """Call a C entry point on device ``gpu``, on that device's current stream. (Launches go to the
     current device; the raw handle spares the 2 us of a Stream object.)"""
     if gpu == torch._C._cuda_getDevice():
-        return fn(args, torch._C._cuda_getCurrentRawStream(gpu))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
     with torch.cuda.device(gpu):
-        return fn(args, torch._C._cuda_getCurrentRawStream(gpu))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
 
 
 def require_cuda(*ts: torch.Tensor) -> None:

@@ -12,7 +12,7 @@ means, scores and lists stands for the i-th block that its new tokens touch, blo
 A step of one layer::
 
     q, pooled_q = rope_append_paged(q, k, v, inv_freq, k_pages, v_pages, table, cu, kv_len, max_new,
-                                    pooled_k=means)
+                                    pooled_k=means, query_mean="new")
     soft = gate.forward_pooled(pooled_q, means, ...).soft_scores
     kept = select_blocks(soft, Hk, cu, kv_len, top_k)
     out = bsa_chunk_paged(q, k_pages, v_pages, table, cu, kv_len, max_new, kept)
@@ -200,6 +200,7 @@ def rope_append_paged(
     interleaved: bool = False,
     attention_scaling: float = 1.0,
     pooled_k: torch.Tensor | None = None,
+    query_mean: str = "block",
     block: int = BLOCK,
     out: torch.Tensor | None = None,
     err: torch.Tensor | None = None,
@@ -212,9 +213,14 @@ def rope_append_paged(
     turn, in pairs ``(i, i + rot/2)`` or, ``interleaved``, ``(2i, 2i + 1)``; cos and sin are multiplied
     by ``attention_scaling``. ``max_new``: most new tokens of a sequence. With ``pooled_k`` (fp32
     ``[B, Hk, NBk, D]``, updated in place: the mean of every key block that got new tokens; one from
-    NBk on is left out and reported in ``err``) also computes the means of the new queries. Returns
-    ``(q, pooled_q)``: rotated q (``out``, which may be q itself; rows outside all sequences are not
-    written) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
+    NBk on is left out and reported in ``err``) also computes the means of the new queries: with
+    ``query_mean="block"`` the sum of a block's new rows over all 64 (the others count as zeros, as the
+    padding behind a whole sequence does where :class:`AttnGate` pools it), with ``"new"`` their own
+    mean. A gate trained on whole sequences has seen means of full blocks: give it ``"new"`` where
+    chunks or single tokens leave blocks in part (a token's sum over 64 hardly moves its scores).
+    Returns ``(q, pooled_q)``: rotated q (``out``, which may be q itself; rows outside all sequences
+    are not written) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for
+    :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
     256. The packed, paged counterpart of :func:`qkv_rope_pool`, which takes cos and sin as tables."""
     name = "rope_append_paged"
     gpu, qs, ks = q.get_device(), q.shape, k_pages.shape
@@ -226,9 +232,9 @@ def rope_append_paged(
             k.get_device() != gpu or v.get_device() != gpu:
         raise KernelError(f"{name}: expects k, v [T, Hk, D] in q's dtype and on its device",
                           context={"q": list(qs), "k": list(k.shape), "v": list(v.shape)})
-    if block != BLOCK or max_new <= 0:
-        raise KernelError(f"{name}: block must be {BLOCK}, max_new positive",
-                          context={"block": block, "max_new": max_new})
+    if block != BLOCK or max_new <= 0 or query_mean not in ("block", "new"):
+        raise KernelError(f"{name}: block must be {BLOCK}, max_new positive, query_mean 'block' or 'new'",
+                          context={"block": block, "max_new": max_new, "query_mean": query_mean})
     f64 = inv_freq.dtype is torch.float64
     if inv_freq.dim() != 1 or not (f64 or inv_freq.dtype is torch.float32) or inv_freq.get_device() != gpu:
         raise KernelError(f"{name}: inv_freq must be [rot / 2], fp64 or fp32, on the same device",
@@ -264,7 +270,7 @@ def rope_append_paged(
         freq.data_ptr(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), pq_ptr, pk_ptr, attention_scaling,
         B, T, Hq, Hk, D, 2 * freq.numel(), block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, rows,
         nbk, interleaved, f64, err_ptr)
-    rc = L.launch(L.lib().tasft_rope_append_paged, args, gpu)
+    rc = L.launch(L.lib().tasft_rope_append_paged_opt, gpu, args, L.ROPE_MEAN_NEW if query_mean == "new" else 0)
     if rc:
         L.check(rc, "tasft_rope_append_paged", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out, pooled_q
@@ -327,7 +333,7 @@ def select_blocks(
         scores.data_ptr(), st[0], st[1], st[2], cu.data_ptr(), kvl.data_ptr(), B, Hq, num_kv_heads, nbq, nbk, block,
         min(top_k, nbk), min(first, nbk), min(local, nbk), tau is not None, 0.0 if tau is None else tau, width,
         idx.data_ptr(), cnt.data_ptr(), err_ptr)
-    rc = L.launch(L.lib().tasft_select_blocks, args, gpu)
+    rc = L.launch(L.lib().tasft_select_blocks, gpu, args)
     if rc:
         L.check(rc, "tasft_select_blocks", shape=[B, Hq, num_kv_heads, nbq, nbk])
     return KeptBlocks(idx, cnt)
@@ -409,7 +415,7 @@ def bsa_chunk_paged(
         *k_pages.stride(), *v_pages.stride(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), idx_ptr, cnt_ptr, B, T, Hq,
         Hk, D, block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, hm, rows, width, scale, ws.data_ptr(),
         nbytes, err_ptr)
-    rc = L.launch(lib.tasft_bsa_chunk_paged_fwd, args, gpu)
+    rc = L.launch(lib.tasft_bsa_chunk_paged_fwd, gpu, args)
     if rc:
         L.check(rc, "tasft_bsa_chunk_paged_fwd", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out

@@ -11,7 +11,8 @@
 //
 // Means are those AttnGate pools (zero padding counts): the sum of a 64-token block's rows as
 // they are held, divided by the block. A key block begun by an earlier call is read back from
-// the cache, so its mean depends only on what the cache holds.
+// the cache, so its mean depends only on what the cache holds. The queries of earlier calls are
+// gone, so with TASFT_ROPE_MEAN_NEW a query mean is over the block's new rows alone.
 //
 // Bound by HBM: every row is read and written once. One CTA of 4 warps takes one 64-token block
 // of one sequence and as many of its heads; a warp takes a head, lanes over (16-byte column
@@ -84,7 +85,7 @@ __device__ __forceinline__ void add_pair(float* acc, const uint4& u1, const uint
 }
 
 template <typename T, bool kMixed>
-__global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasft_rope_append_args a) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasft_rope_append_args a, const int options) {
   constexpr int V = Vec16<T>::N;
   // [row][float4 of cos, then of sin][column pair]: the lanes of a row read 16 bytes beside one another
   extern __shared__ __align__(16) float trig[];
@@ -247,21 +248,23 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasf
       }
     }
     if (r0 == 0) {
+      // (1 / 64 is exact: the same bits as a division)
+      const float inv = is_q && (options & TASFT_ROPE_MEAN_NEW) ? 1.f / (r_hi - r_lo) : 1.f / kRopeBlk;
       float* dst = is_q ? a.pooled_q + (((int64_t)b * a.Hq + hh) * a.NBq + qi) * a.D
                         : a.pooled_k + (((int64_t)b * a.Hk + hh) * a.NBk + blk) * a.D;
 #pragma unroll
       for (int i = 0; i < V; i += 4) {
         *reinterpret_cast<float4*>(dst + c1 + i) =
-            make_float4(acc[i] / kRopeBlk, acc[i + 1] / kRopeBlk, acc[i + 2] / kRopeBlk, acc[i + 3] / kRopeBlk);
-        *reinterpret_cast<float4*>(dst + c2 + i) = make_float4(acc[V + i] / kRopeBlk, acc[V + i + 1] / kRopeBlk,
-                                                               acc[V + i + 2] / kRopeBlk, acc[V + i + 3] / kRopeBlk);
+            make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+        *reinterpret_cast<float4*>(dst + c2 + i) =
+            make_float4(acc[V + i] * inv, acc[V + i + 1] * inv, acc[V + i + 2] * inv, acc[V + i + 3] * inv);
       }
     }
   }
 }
 
 template <typename T, bool kMixed>
-int run(const tasft_rope_append_args& a, cudaStream_t st) {
+int run(const tasft_rope_append_args& a, int options, cudaStream_t st) {
   auto kern = rope_append_kernel<T, kMixed>;
   const int smem = kRopeRows * a.rot * (int)sizeof(float);  // cos and sin, rot / 2 each
   constexpr int kPlaces = 2 * kRopeBlk * (int)sizeof(int64_t);  // static, and counted against the limit too
@@ -269,7 +272,7 @@ int run(const tasft_rope_append_args& a, cudaStream_t st) {
   if (smem + kPlaces > 48 * 1024 && !allow_smem(kern, kRopeRows * 256 * (int)sizeof(float), allowed)) return TASFT_ERR_CUDA;
   const int z = (a.Hq + 2 * a.Hk + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
   if (a.B > 65535) return TASFT_ERR_TOO_LARGE;
-  kern<<<dim3((unsigned)z, (unsigned)a.NBq, (unsigned)a.B), kRopeThreads, smem, st>>>(a);
+  kern<<<dim3((unsigned)z, (unsigned)a.NBq, (unsigned)a.B), kRopeThreads, smem, st>>>(a, options);
   count_launch();
   return launch_status();
 }
@@ -287,7 +290,11 @@ bool rows_ok(const void* p, const int64_t* st, int n, int per16) {
 using namespace tasft;
 
 extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_stream_t stream) {
-  if (!ap) return TASFT_ERR_INVALID_ARG;
+  return tasft_rope_append_paged_opt(ap, 0, stream);
+}
+
+extern "C" int tasft_rope_append_paged_opt(const tasft_rope_append_args* ap, int32_t options, tasft_stream_t stream) {
+  if (!ap || (options & ~TASFT_ROPE_MEAN_NEW)) return TASFT_ERR_INVALID_ARG;
   tasft_rope_append_args a = *ap;
   // strides of axes of length one say nothing
   if (a.T <= 1) a.q_stride[0] = a.k_in_stride[0] = a.v_in_stride[0] = a.o_stride[0] = 0;
@@ -318,7 +325,7 @@ extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_s
     return TASFT_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool mixed = a.interleaved != 0;
-  if (a.dtype == TASFT_F32) return mixed ? run<float, true>(a, st) : run<float, false>(a, st);
-  if (a.dtype == TASFT_F16) return mixed ? run<__half, true>(a, st) : run<__half, false>(a, st);
-  return mixed ? run<__nv_bfloat16, true>(a, st) : run<__nv_bfloat16, false>(a, st);
+  if (a.dtype == TASFT_F32) return mixed ? run<float, true>(a, options, st) : run<float, false>(a, options, st);
+  if (a.dtype == TASFT_F16) return mixed ? run<__half, true>(a, options, st) : run<__half, false>(a, options, st);
+  return mixed ? run<__nv_bfloat16, true>(a, options, st) : run<__nv_bfloat16, false>(a, options, st);
 }

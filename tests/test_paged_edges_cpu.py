@@ -102,3 +102,12 @@ def test_options_that_would_change_the_result_are_not_dropped(scaling):
 def test_numbers_without_a_meaning_are_refused(args):
     with pytest.raises(T.ValidationError):
         T.rope_inv_freq(*args)
+
+
+def test_options_that_are_not_known_are_refused():
+    a = L.RopeAppendArgs(q=4096, k=4096, v=4096, q_out=4096, k_pages=4096, v_pages=4096, inv_freq=4096,
+                         block_table=4096, cu_seqlens=4096, kv_len=4096, factor=1.0, B=2, T=5, Hq=8, Hk=2, D=128, rot=128,
+                         block=64, dtype=L.BF16, max_q=4, max_pages=4, page_size=16, num_pages=9, NBq=2, NBk=4)
+    for options in (1 << 10, -1):
+        assert L.lib().tasft_rope_append_paged_opt(C.byref(a), options, None) == -1
+    assert L.lib().tasft_rope_append_paged_opt(None, 0, None) == -1

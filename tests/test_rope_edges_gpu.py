@@ -85,3 +85,70 @@ def test_rows_without_a_page_take_no_part_in_a_mean(dtype):
         # 63 fp32 additions, each at most half a step off
         tol = 64 * 2.0 ** -24 * held.abs().sum(0) / 64
         assert ((means[0, :, 0].double() - held.sum(0) / 64).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("new,ctx", [([1], [0]), ([1], [100]), ([37, 1, 0, 150], [50, 63, 0, 20]), ([64, 63], [64, 1])])
+def test_means_over_the_new_queries_alone(dtype, new, ctx):
+    q, k, v, freq, kp, vp, table, cu, kv_len = batch(new, ctx, 6, 2, 64, 16, dtype, seed=2)
+    nbk = max((n + c + 63) // 64 for n, c in zip(new, ctx))
+    means = [torch.zeros(len(new), 2, nbk, 64, device=DEV) for _ in range(2)]
+    args = (q, k, v, freq, kp, vp, table, cu, kv_len, max(new))
+    out, pooled = T.rope_append_paged(*args, pooled_k=means[0], query_mean="new")
+    _, padded = T.rope_append_paged(*args, pooled_k=means[1])
+    assert torch.equal(means[0], means[1])  # key means are over what the cache holds either way
+    at = 0
+    for b, (n, c) in enumerate(zip(new, ctx)):
+        for i in range(pooled.shape[2]):
+            lo, hi = max((c // 64 + i) * 64, c) - c, min((c // 64 + i + 1) * 64, c + n) - c
+            if hi <= lo:
+                assert (pooled[b, :, i] == 0).all() and (padded[b, :, i] == 0).all()
+                continue
+            rows = out[at + lo:at + hi].double()
+            # 63 fp32 additions, 1 / rows and the product, each at most half a step off
+            tol = 66 * 2.0 ** -24 * rows.abs().mean(0)
+            assert ((pooled[b, :, i].double() - rows.mean(0)).abs() <= tol).all()
+            if hi - lo == 1:
+                assert torch.equal(pooled[b, :, i], out[at + lo].float())
+            if hi - lo == 64:
+                assert torch.equal(pooled[b, :, i], padded[b, :, i])
+        at += n
+
+
+def test_query_mean_is_one_of_two():
+    args = batch([3], [5], 4, 2, 64, 16, torch.bfloat16)
+    with pytest.raises(T.KernelError):
+        T.rope_append_paged(*args, 3, query_mean="rows")
+
+
+def test_chunks_of_whole_blocks_choose_as_the_whole_prompt_does():
+    """The gate's lists for a prompt do not depend on how it was cut, as long as blocks stay whole; in a
+    cut one every row of its parts still has a mean of full weight."""
+    Hq, Hk, D, n = 8, 2, 128, 700
+    q, k, v, freq, kp, vp, table, cu, kv_len = batch([n], [0], Hq, Hk, D, 16, torch.bfloat16, seed=5)
+    torch.manual_seed(5)
+    gate = T.AttnGate(Hq, D, block_size=64, is_causal=False).to(DEV)
+    torch.nn.init.normal_(gate.gate_proj_out.weight, std=1.0)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+
+    def lists(cuts):
+        means, got, weight = torch.zeros(1, Hk, 11, D, device=DEV), {}, []
+        for lo, hi in zip(cuts[:-1], cuts[1:]):
+            c, m = ints(0, hi - lo), hi - lo
+            _, pooled = T.rope_append_paged(q[lo:hi], k[lo:hi], v[lo:hi], freq, kp, vp, table, c, ints(hi), m, pooled_k=means,
+                                            query_mean="new")
+            with torch.no_grad():
+                soft = gate.forward_pooled(pooled, means, pooled.shape[2] * 64, 11 * 64).soft_scores
+            kept = T.select_blocks(soft, Hk, c, ints(hi), 4)
+            for i in range((hi - 1) // 64 - lo // 64 + 1):
+                got[lo // 64 + i, lo] = kept.idx[0, :, i].tolist()
+                weight.append(pooled[0, :, i].abs().mean().item())
+        return got, weight
+
+    whole, _ = lists([0, n])
+    for cuts in ([0, 64, 320, n], [0, 384, 448, n]):
+        got, _ = lists(cuts)
+        assert {key[0]: x for key, x in got.items()} == {key[0]: x for key, x in whole.items()}
+    _, weight = lists([0, 100, 101, 300, n])
+    _, full = lists([0, 640])
+    assert min(weight) >= 0.9 * min(full)  # (a mean of fewer random rows is larger, a sum over 64 smaller)
