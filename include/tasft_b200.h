@@ -23,7 +23,7 @@
  *                              tasft/modules/tasft_attention.py:615-742, attn_gate.py:351-375
  *   tasft_rope_append_paged    (none: the paged, packed form of tasft_qkv_rope_pool); _opt
  *   tasft_select_blocks        (none: top-scored blocks; the reference keeps by threshold)
- *   tasft_bsa_chunk_paged_fwd  (none: the reference's vLLM prefill has no cache behind it,
+ *   tasft_bsa_chunk_paged_fwd, _opt  (none: the reference's vLLM prefill has no cache behind it,
  *                              tasft/inference/vllm_patch.py:172-196)
  *   tasft_mask_to_kept         bool mask & block tril     tasft/kernels/block_sparse_fa.py:497-508
  *   tasft_calibrate_tau        the weight-norm estimate of per-layer sparsity
@@ -411,6 +411,12 @@ typedef struct {
 TASFT_API int64_t tasft_chunk_workspace_size(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q,
                                              int32_t Hm);  /* Hm 0: no lists */
 TASFT_API int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* args, tasft_stream_t stream);
+
+/* The same with options (0: the call above). TASFT_ZERO_REST: rows of out that no sequence accounts
+ * for (outside all of them, or of one that does not fit) are set to 0, for a tensor that holds
+ * nothing yet. */
+#define TASFT_ZERO_REST 2
+TASFT_API int tasft_bsa_chunk_paged_fwd_opt(const tasft_chunk_args* args, int32_t options, tasft_stream_t stream);
 
 /* Merge G partial results (normalised o, m, l) into the final output. */
 typedef struct {

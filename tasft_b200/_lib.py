@@ -118,7 +118,9 @@ class PagedDecodeArgs(C.Structure):
 I64x2 = C.c_int64 * 2
 
 
-ROPE_MEAN_NEW = 1  # options of tasft_rope_append_paged_opt
+# options of the _opt calls
+ROPE_MEAN_NEW = 1
+ZERO_REST = 2
 
 
 class RopeAppendArgs(C.Structure):
@@ -224,6 +226,7 @@ SIGNATURES = {
     "tasft_select_blocks": ([vp, vp], C.c_int),
     "tasft_chunk_workspace_size": ([C.c_int32] * 7, C.c_int64),
     "tasft_bsa_chunk_paged_fwd": ([vp, vp], C.c_int),
+    "tasft_bsa_chunk_paged_fwd_opt": ([vp, C.c_int32, vp], C.c_int),
     "tasft_mask_to_kept": ([C.POINTER(MaskArgs), vp], C.c_int),
     "tasft_calibrate_tau": ([C.POINTER(CalibArgs), vp], C.c_int),
     "tasft_bsa_prefill_fwd": ([C.POINTER(PrefillArgs), vp], C.c_int),

@@ -361,9 +361,10 @@ def bsa_chunk_paged(
     q ``[T, Hq, D]``, pages ``[num_pages, page_size, Hk, D]`` with the new keys and values already
     in them (:func:`rope_append_paged`), ``kept`` lists ``[B, Hk or Hq, NBq, W]`` with at least
     ``chunk_rows(max_new)`` rows, ascending. ``scale`` defaults to ``1 / sqrt(D)``. Returns
-    ``[T, Hq, D]`` (``out``, which may be q itself; rows outside all sequences stay as they were, undefined in a new
-    tensor); a token with nothing kept gets 0. ``err``: optional int32 error word, see ``include/tasft_b200.h``. bf16 / f16, D 64
-    or 128, page size 16, 32, 64 or 128. What the cache holds from ``kv_len`` on, behind a
+    ``[T, Hq, D]``: a new tensor, 0 in rows that no sequence accounts for (outside all of them, or of
+    one whose lengths do not fit), or ``out``, which may be q itself and where such rows stay as they
+    were. A token with nothing kept gets 0. ``err``: optional int32 error word, see
+    ``include/tasft_b200.h``. bf16 / f16, D 64 or 128, page size 16, 32, 64 or 128. What the cache holds from ``kv_len`` on, behind a
     token's own position or in blocks its list does not keep never reaches its row, infinities
     and NaN neither. Beside :func:`bsa_decode_paged` (one token per sequence) and
     :meth:`BlockSparseFlashAttention.forward_varlen` (no cache)."""
@@ -397,15 +398,17 @@ def bsa_chunk_paged(
             cnt = cnt.to(torch.int32).contiguous()
         idx_ptr, cnt_ptr = idx.data_ptr(), cnt.data_ptr()
         _, hm, rows, width = ls
+    if gpu != torch._C._cuda_getDevice():  # the workspace is sized for the current device
+        with torch.cuda.device(gpu):
+            return bsa_chunk_paged(q, k_pages, v_pages, table, cu, kvl, max_new, kept, block, scale=scale, out=out, err=err)
+    options = 0
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        options = L.ZERO_REST
     elif out.shape != qs or out.dtype is not q.dtype or out.get_device() != gpu or out.stride(2) != 1:
         raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
     q, st = _rows(q, 8)
     lib = L.lib()
-    if gpu != torch._C._cuda_getDevice():  # the workspace is sized for the current device
-        with torch.cuda.device(gpu):
-            return bsa_chunk_paged(q, k_pages, v_pages, table, cu, kvl, max_new, kept, block, scale=scale, out=out, err=err)
     nbytes = lib.tasft_chunk_workspace_size(B, T, Hq, Hk, D, max_new, hm)
     if nbytes < 0:
         L.check(int(nbytes), "tasft_chunk_workspace_size", shape=[B, T, Hq, Hk, D])
@@ -415,7 +418,7 @@ def bsa_chunk_paged(
         *k_pages.stride(), *v_pages.stride(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), idx_ptr, cnt_ptr, B, T, Hq,
         Hk, D, block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, hm, rows, width, scale, ws.data_ptr(),
         nbytes, err_ptr)
-    rc = L.launch(lib.tasft_bsa_chunk_paged_fwd, gpu, args)
+    rc = L.launch(lib.tasft_bsa_chunk_paged_fwd_opt, gpu, args, options)
     if rc:
         L.check(rc, "tasft_bsa_chunk_paged_fwd", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out

@@ -22,6 +22,7 @@ struct ChunkShape {
   int stride;     // sequences per entry of the table
   int may_cut;    // 0: cutting tiles gains nothing
   int wide;       // rows of out on 32-byte boundaries
+  int zero_rest;  // rows of out that no sequence accounts for become 0
 };
 
 struct ChunkSeq {
@@ -39,17 +40,20 @@ __device__ __forceinline__ int chunk_tiles(const ChunkShape& sh, int n, int ctx,
   return ((len - 1) >> sh.tpt_log2) - (ctx >> sh.tpt_log2) + 1;
 }
 
+// Whether sequence rows and lengths fit T, max_q, the block table and each other.
+__device__ __forceinline__ bool chunk_fits(const tasft_chunk_args& a, const ChunkShape& sh, int start, int end, int len) {
+  if (start < 0 || end < start || end > a.T) return false;
+  const int n = end - start;
+  return n == 0 || (len >= n && len <= sh.capacity && n <= a.max_q);
+}
+
 __device__ __forceinline__ ChunkSeq chunk_seq(const tasft_chunk_args& a, const ChunkShape& sh, int b) {
   ChunkSeq s;
   s.start = a.cu_seqlens[b];
   const int end = a.cu_seqlens[b + 1];
   s.len = a.kv_len[b];
-  s.bad = s.start < 0 || end < s.start || end > a.T;
+  s.bad = !chunk_fits(a, sh, s.start, end, s.len);
   s.n = s.bad ? 0 : end - s.start;
-  if (s.n > 0 && (s.len < s.n || s.len > sh.capacity || s.n > a.max_q)) {
-    s.bad = true;
-    s.n = 0;
-  }
   s.ctx = s.n > 0 ? s.len - s.n : 0;
   s.tiles = chunk_tiles(sh, s.n, s.ctx, s.len);
   s.cost = 0;

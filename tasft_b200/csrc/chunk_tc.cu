@@ -302,6 +302,30 @@ __global__ void __launch_bounds__(kThreads, 2)
       fetch(a.kept_cnt, (int64_t)a.B * a.Hm * a.nb_q * 4);
       fetch(a.kept_idx, (int64_t)a.B * a.Hm * a.nb_q * a.nb_w * 4);
     }
+    if (sh.zero_rest) {  // beside warp 2's count, a share of the rows per CTA
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      auto zero = [&](int from, int to) {
+        constexpr int kPieces = D / 8;  // of 16 bytes, of a head's row
+        for (int64_t r = (int64_t)from + blockIdx.x; r < to; r += gridDim.x)
+          for (int i = lane; i < a.Hq * kPieces; i += 32)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + r * a.o_stride[0] +
+                                      (i / kPieces) * a.o_stride[1] + (i % kPieces) * 8) = make_uint4(0, 0, 0, 0);
+      };
+      auto within = [&](int r) { return max(0, min(r, a.T)); };
+      // before the first sequence, behind the last one, and those that do not fit
+      zero(0, within(a.cu_seqlens[0]));
+      zero(within(a.cu_seqlens[a.B]), a.T);
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + lane;
+        unsigned left_out = __ballot_sync(
+            0xffffffffu, b < a.B && !chunk_fits(a, sh, a.cu_seqlens[b], a.cu_seqlens[b + 1], a.kv_len[b]));
+        for (; left_out; left_out &= left_out - 1) {
+          const int bad = b0 + __ffs(left_out) - 1;
+          zero(within(a.cu_seqlens[bad]), within(a.cu_seqlens[bad + 1]));
+        }
+      }
+      __syncwarp();
+    }
   }
   int64_t* before = reinterpret_cast<int64_t*>(smem + L::kSumOff);  // weight before a bucket's first sequence
   int4* seqs = reinterpret_cast<int4*>(smem + L::kSeqOff);          // start, n, len, cost (stride 1)
@@ -1376,13 +1400,17 @@ using namespace tasft;
 extern "C" int64_t tasft_chunk_workspace_size(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q,
                                               int32_t Hm) {
   if (B <= 0 || T < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D <= 0 || max_q <= 0 || Hm < 0) return TASFT_ERR_INVALID_ARG;
-  ChunkShape sh;
+  ChunkShape sh = {};
   if (!chunk_shape(sh, Hq, Hk, Hm, max_q)) return TASFT_ERR_UNSUPPORTED;
   return ws_layout(sh, D, 2 * sm_count()).bytes;
 }
 
 extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_stream_t stream) {
-  if (!ap) return TASFT_ERR_INVALID_ARG;
+  return tasft_bsa_chunk_paged_fwd_opt(ap, 0, stream);
+}
+
+extern "C" int tasft_bsa_chunk_paged_fwd_opt(const tasft_chunk_args* ap, int32_t options, tasft_stream_t stream) {
+  if (!ap || (options & ~TASFT_ZERO_REST)) return TASFT_ERR_INVALID_ARG;
   tasft_chunk_args a = *ap;
   // strides of axes of length one say nothing
   if (a.T == 1) a.q_stride[0] = a.o_stride[0] = a.D;
@@ -1415,6 +1443,7 @@ extern "C" int tasft_bsa_chunk_paged_fwd(const tasft_chunk_args* ap, tasft_strea
   if (a.kept_idx && (int64_t)a.nb_w * 2 < bound) bound = a.nb_w * (sh.mode == 2 ? 2 : 1);
   // 32-byte stores of out's rows
   sh.wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.o_stride[0] % 16 == 0 && a.o_stride[1] % 16 == 0;
+  sh.zero_rest = (options & TASFT_ZERO_REST) != 0;
   sh.stride = (a.B + kChunkBuckets - 1) / kChunkBuckets;
   // One launch where cutting tiles gains nothing (the device decides the rest). Tiles with lists
   // take about as long as one another: the gain is the last round's idle share of the longest, for

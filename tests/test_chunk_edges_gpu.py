@@ -78,3 +78,78 @@ def test_many_small_probabilities_in_half_precision(ctx, D, top):
     # against a sum of at least 1, and 2^-14 for fp32 scores, exponentials and sums, as in attend_bound
     bound = 2.0 ** -11 * o.abs() + 2.0 ** -14 * a + n * 2.0 ** -31 * vp.max().item() + 2.0 ** -25
     assert ((out.double() - o).abs() <= bound).all()
+
+
+def packed(new, ctx, D=128, page=16, seed=7):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    kp, vp, table, cu, kv_len = R.layout(new, ctx, page, 2, D, torch.bfloat16, DEV, g)
+    q = torch.randn(sum(new) + 9, 8, D, generator=g, device=DEV).to(torch.bfloat16)
+    return q, kp, vp, table, cu, kv_len, g
+
+
+def used_memory(like):
+    """Leaves values where the next tensor of this size is likely to come."""
+    torch.full_like(like, 7.0, memory_format=torch.contiguous_format)
+
+
+@pytest.mark.parametrize("lists", [None, "kv", "q"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_that_no_sequence_accounts_for_are_zero_in_a_new_tensor(lists, D):
+    """Padding before and behind the sequences, a sequence that does not fit, all of them: 0 in a new
+    tensor, left as they were in one that is given; the other rows as ever."""
+    new, ctx = [40, 1, 0, 70, 5], [300, 900, 0, 0, 64]
+    q, kp, vp, table, cu, kv_len, g = packed(new, ctx, D)
+    kept = None
+    if lists:
+        kept = T.KeptBlocks(*R.random_lists(new, ctx, 2 if lists == "kv" else 8, 15, DEV, g, 0.6))
+    cu = cu + 3  # three rows before, six behind
+    good = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, 70, kept)
+    o, a = R.attend(q[3:119], kp, vp, table, new, ctx, None if kept is None else (kept.idx, kept.cnt))
+    assert ((good[3:119].double() - o).abs() <= R.attend_bound(o, a, torch.bfloat16, 901)).all()
+    for gone in ([], [0], [1, 4], [3], [0, 1, 3, 4]):
+        n = kv_len.clone()
+        n[gone] = 10 ** 6
+        dead = torch.ones(q.shape[0], dtype=torch.bool, device=DEV)
+        for b in range(5):
+            if b not in gone:
+                dead[int(cu[b]):int(cu[b + 1])] = False
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        used_memory(q)
+        out = T.bsa_chunk_paged(q, kp, vp, table, cu, n, 70, kept, err=err)
+        assert int(err.item()) == (1 if gone else 0)
+        assert (out[dead] == 0).all() and torch.isfinite(out).all()
+        o_dead, a_dead = o.clone(), a.clone()
+        live = ~dead[3:119]
+        assert ((out[3:119].double() - o_dead).abs()[live] <= R.attend_bound(o_dead, a_dead, torch.bfloat16, 901)[live]).all()
+        mine = torch.full_like(q, 3.0)
+        T.bsa_chunk_paged(q, kp, vp, table, cu, n, 70, kept, out=mine)
+        assert (mine[dead] == 3).all() and torch.equal(mine[~dead], out[~dead])
+
+
+@pytest.mark.parametrize("cu", [[0, 4, 90, 12, 20], [-4, 4, 8, 12, 16], [30, 20, 10, 4, 0], [0, 0, 0, 0, 0],
+                                [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, 9]])
+def test_row_ranges_that_make_no_sense_leave_nothing_unset(cu):
+    q, kp, vp, table, _, kv_len, g = packed([4, 4, 4, 4], [50, 60, 70, 0])
+    used_memory(q)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = T.bsa_chunk_paged(q, kp, vp, table, torch.tensor(cu, device=DEV).to(torch.int32), kv_len, 4, err=err)
+    assert torch.isfinite(out).all() and (out != 7).all()
+    assert int(err.item()) == (0 if cu == [0] * 5 else 1)
+
+
+def test_padding_of_a_captured_step_follows_the_lengths():
+    q, kp, vp, table, cu, kv_len, g = packed([33, 1, 1], [500, 900, 40])
+    T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, 33)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = T.bsa_chunk_paged(q, kp, vp, table, cu, kv_len, 33)
+    for new in ([33, 1, 1], [2, 7, 0], [0, 0, 0], [30, 5, 9]):
+        cu.copy_(torch.tensor([sum(new[:b]) for b in range(4)], dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        n = sum(new)
+        assert (out[n:] == 0).all()
+        total = kv_len.tolist()
+        o, a = R.attend(q[:n], kp, vp, table, new, [t - m for t, m in zip(total, new)])
+        assert ((out[:n].double() - o).abs() <= R.attend_bound(o, a, torch.bfloat16, 901)).all()

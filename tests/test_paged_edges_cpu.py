@@ -110,4 +110,5 @@ def test_options_that_are_not_known_are_refused():
                          block=64, dtype=L.BF16, max_q=4, max_pages=4, page_size=16, num_pages=9, NBq=2, NBk=4)
     for options in (1 << 10, -1):
         assert L.lib().tasft_rope_append_paged_opt(C.byref(a), options, None) == -1
-    assert L.lib().tasft_rope_append_paged_opt(None, 0, None) == -1
+        assert L.lib().tasft_bsa_chunk_paged_fwd_opt(C.byref(chunk_args()), options, None) == -1
+    assert L.lib().tasft_rope_append_paged_opt(None, 0, None) == L.lib().tasft_bsa_chunk_paged_fwd_opt(None, 0, None) == -1
