@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasf
   const int half = a.rot / 2;
   const int start = a.cu_seqlens[b], end = a.cu_seqlens[b + 1], len = a.kv_len[b];
   const int n = end - start;
-  const bool bad = start < 0 || n < 0 || end > a.T ||
+  // (end < start, not n < 0: the difference may leave 32 bits)
+  const bool bad = start < 0 || end < start || end > a.T ||
                    (n > 0 && (len < n || len > (int64_t)a.max_pages * a.page_size || n > a.max_q));
   const int ctx = len - n;
   const int blk = bad || n == 0 ? 0 : ctx / kRopeBlk + qi;

@@ -152,3 +152,24 @@ def test_chunks_of_whole_blocks_choose_as_the_whole_prompt_does():
     _, weight = lists([0, 100, 101, 300, n])
     _, full = lists([0, 640])
     assert min(weight) >= 0.9 * min(full)  # (a mean of fewer random rows is larger, a sum over 64 smaller)
+
+
+@pytest.mark.parametrize("cu", [[0, 4, 90, 12, 20], [-4, 4, 8, 12, 16], [30, 20, 10, 4, 0],
+                                [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, 9], [1, -2 ** 31, 4, 5, 3]])
+def test_row_ranges_that_make_no_sense_are_left_out(cu):
+    """Ends before starts by so much that their difference wraps to a small number among them."""
+    q, k, v, freq, kp, vp, table, _, kv_len = batch([4, 4, 4, 13], [50, 60, 70, 0], 6, 2, 64, 16, torch.bfloat16)
+    k1, v1, out = kp.clone(), vp.clone(), torch.full_like(q, 7.0, memory_format=torch.contiguous_format)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    T.rope_append_paged(q, k, v, freq, k1, v1, table, torch.tensor(cu, device=DEV).to(torch.int32), kv_len, 4, out=out,
+                        err=err)
+    assert int(err.item()) == 1
+    fits = [0 <= cu[b] <= cu[b + 1] <= 25 and cu[b + 1] - cu[b] <= 4 for b in range(4)]
+    row = torch.zeros(25, dtype=torch.bool, device=DEV)
+    page = torch.zeros(kp.shape[0], dtype=torch.bool, device=DEV)
+    for b in range(4):
+        if fits[b]:
+            row[cu[b]:cu[b + 1]] = True
+            page[table[b][table[b] >= 0].long()] = True
+    assert (out[~row] == 7).all()
+    assert torch.equal(k1[~page], kp[~page]) and torch.equal(v1[~page], vp[~page])
