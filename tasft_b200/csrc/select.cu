@@ -56,8 +56,9 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) select_blocks_kernel(cons
   int32_t* idx = a.kept_idx + row * a.width;
   const int grp = a.Hq / a.Hk;
 
-  const int n_new = a.cu_seqlens[b + 1] - a.cu_seqlens[b], len = a.kv_len[b];
-  const int own0 = (len - n_new) >> log2_block, own_last = (len - 1) >> log2_block;
+  const int len = a.kv_len[b];
+  const int64_t n_new = (int64_t)a.cu_seqlens[b + 1] - a.cu_seqlens[b];  // (may leave 32 bits)
+  const int own0 = (int)((len - n_new) >> log2_block), own_last = (len - 1) >> log2_block;
   const bool bad = n_new < 0 || (n_new > 0 && (len < n_new || own_last >= a.NBk || own_last - own0 >= a.NBq));
   const int mine = own0 + i;
   if (bad || n_new <= 0 || mine > own_last) {  // no such row
