@@ -186,7 +186,8 @@ typedef struct {
 } tasft_rope_append_args;
 TASFT_API int tasft_rope_append_paged(const tasft_rope_append_args* args, tasft_stream_t stream);
 
-/* The same with options (0: the call above). TASFT_ROPE_MEAN_NEW: a row of pooled_q is the mean
+/* The same with options (0: the call above). TASFT_ZERO_REST: rows of q_out that no sequence accounts
+ * for are set to 0 (see tasft_bsa_chunk_paged_fwd_opt). TASFT_ROPE_MEAN_NEW: a row of pooled_q is the mean
  * over the block's new rows, not their sum over the block. A gate that was trained on whole
  * sequences saw means of full blocks; a single token's sum over 64 is next to nothing to it, and the
  * rest of the block's queries are gone. */

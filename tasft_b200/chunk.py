@@ -218,9 +218,9 @@ def rope_append_paged(
     padding behind a whole sequence does where :class:`AttnGate` pools it), with ``"new"`` their own
     mean. A gate trained on whole sequences has seen means of full blocks: give it ``"new"`` where
     chunks or single tokens leave blocks in part (a token's sum over 64 hardly moves its scores).
-    Returns ``(q, pooled_q)``: rotated q (``out``, which may be q itself; rows outside all sequences
-    are not written) and fp32 ``[B, Hq, chunk_rows(max_new), D]`` or None, for
-    :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
+    Returns ``(q, pooled_q)``: rotated q (a new tensor, 0 in rows that no sequence accounts for, or
+    ``out``, which may be q itself and where such rows are not written) and fp32 ``[B, Hq,
+    chunk_rows(max_new), D]`` or None, for :meth:`AttnGate.forward_pooled`. f32 / bf16 / f16; D and rot multiples of 16 (8 in f32), D up to
     256. The packed, paged counterpart of :func:`qkv_rope_pool`, which takes cos and sin as tables."""
     name = "rope_append_paged"
     gpu, qs, ks = q.get_device(), q.shape, k_pages.shape
@@ -257,8 +257,10 @@ def rope_append_paged(
         nbk = ps[2]
         pooled_q = torch.empty(B, Hq, rows, D, dtype=torch.float32, device=dev)
         pq_ptr, pk_ptr = pooled_q.data_ptr(), pooled_k.data_ptr()
+    options = L.ROPE_MEAN_NEW if query_mean == "new" else 0
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        options |= L.ZERO_REST
     elif out.shape != qs or out.dtype is not dtype or out.get_device() != gpu or out.stride(2) != 1:
         raise KernelError(f"{name}: out must match q", context={"q": list(qs), "out": list(out.shape)})
     per16 = 16 // dtype.itemsize
@@ -270,7 +272,7 @@ def rope_append_paged(
         freq.data_ptr(), table.data_ptr(), cu.data_ptr(), kvl.data_ptr(), pq_ptr, pk_ptr, attention_scaling,
         B, T, Hq, Hk, D, 2 * freq.numel(), block, L.dtype_code(q), max_new, table.size(1), page_size, num_pages, rows,
         nbk, interleaved, f64, err_ptr)
-    rc = L.launch(L.lib().tasft_rope_append_paged_opt, gpu, args, L.ROPE_MEAN_NEW if query_mean == "new" else 0)
+    rc = L.launch(L.lib().tasft_rope_append_paged_opt, gpu, args, options)
     if rc:
         L.check(rc, "tasft_rope_append_paged", shape=[B, T, Hq, Hk, D], page_size=page_size)
     return out, pooled_q

@@ -104,6 +104,18 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const tasf
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = a.Hq + 2 * a.Hk;
   const int h = blockIdx.x * (kRopeThreads / 32) + warp;
+  if ((options & TASFT_ZERO_REST) && h < a.Hq) {  // rows of q_out that no sequence accounts for
+    auto zero = [&](int from, int to) {
+      T* row = reinterpret_cast<T*>(a.q_out) + h * a.o_stride[1];
+      for (int64_t r = (int64_t)from + qi; r < to; r += gridDim.y)
+        for (int d = lane * V; d < a.D; d += 32 * V)
+          *reinterpret_cast<uint4*>(row + r * a.o_stride[0] + d) = make_uint4(0, 0, 0, 0);
+    };
+    const int lo = max(0, min(start, a.T)), hi = max(0, min(end, a.T));
+    if (b == 0) zero(0, lo);
+    if (b == a.B - 1) zero(hi, a.T);
+    if (bad) zero(lo, hi);
+  }
   if (!there) {
     if (bad && qi == 0 && blockIdx.x == 0 && threadIdx.x == 0) set_err(a.err, TASFT_DEVERR_INDEX);
     if (a.pooled_q && h < a.Hq)  // a row that no new token falls in has a mean of zero
@@ -295,7 +307,7 @@ extern "C" int tasft_rope_append_paged(const tasft_rope_append_args* ap, tasft_s
 }
 
 extern "C" int tasft_rope_append_paged_opt(const tasft_rope_append_args* ap, int32_t options, tasft_stream_t stream) {
-  if (!ap || (options & ~TASFT_ROPE_MEAN_NEW)) return TASFT_ERR_INVALID_ARG;
+  if (!ap || (options & ~(TASFT_ROPE_MEAN_NEW | TASFT_ZERO_REST))) return TASFT_ERR_INVALID_ARG;
   tasft_rope_append_args a = *ap;
   // strides of axes of length one say nothing
   if (a.T <= 1) a.q_stride[0] = a.k_in_stride[0] = a.v_in_stride[0] = a.o_stride[0] = 0;

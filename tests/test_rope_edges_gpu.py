@@ -173,3 +173,42 @@ def test_row_ranges_that_make_no_sense_are_left_out(cu):
             page[table[b][table[b] >= 0].long()] = True
     assert (out[~row] == 7).all()
     assert torch.equal(k1[~page], kp[~page]) and torch.equal(v1[~page], vp[~page])
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 256), (torch.float32, 128)])
+def test_rows_that_no_sequence_accounts_for_are_zero_in_a_new_tensor(dtype, D):
+    """Padding before and behind the sequences, a sequence that does not fit: 0 in a new tensor, left as
+    they were in one that is given."""
+    new, ctx = [40, 1, 0, 170, 5], [30, 90, 0, 0, 64]
+    g = torch.Generator(device=DEV).manual_seed(4)
+    kp, vp, table, cu, kv_len = R.layout(new, ctx, 16, 2, D, dtype, DEV, g)
+    rows = torch.randn(sum(new) + 9, 10, D, generator=g, device=DEV).to(dtype)
+    q, k, v = rows[:, :6], rows[:, 6:8], rows[:, 8:]
+    freq, _ = T.rope_inv_freq(D, device=DEV)
+    cu = cu + 3
+    want = None
+    for gone in ([], [0], [1, 4], [3], [0, 1, 3, 4]):
+        n = kv_len.clone()
+        n[gone] = 10 ** 6
+        dead = torch.ones(rows.shape[0], dtype=torch.bool, device=DEV)
+        for b in range(5):
+            if b not in gone:
+                dead[int(cu[b]):int(cu[b + 1])] = False
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        torch.full_like(q, 7.0, memory_format=torch.contiguous_format)  # where the new tensor is likely to come
+        out, _ = T.rope_append_paged(q, k, v, freq, kp, vp, table, cu, n, 170, err=err)
+        assert int(err.item()) == (1 if gone else 0)
+        want = out.clone() if want is None else want
+        assert (out[dead] == 0).all() and torch.equal(out[~dead], want[~dead])
+        mine = torch.full((rows.shape[0], 6, D), 3.0, device=DEV, dtype=dtype)
+        T.rope_append_paged(q, k, v, freq, kp, vp, table, cu, n, 170, out=mine)
+        assert (mine[dead] == 3).all() and torch.equal(mine[~dead], want[~dead])
+
+
+@pytest.mark.parametrize("cu", [[0, 4, 90, 12, 20], [-4, 4, 8, 12, 16], [30, 20, 10, 4, 0], [0, 0, 0, 0, 0],
+                                [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, 9]])
+def test_row_ranges_that_make_no_sense_leave_nothing_unset(cu):
+    q, k, v, freq, kp, vp, table, _, kv_len = batch([4, 4, 4, 13], [50, 60, 70, 0], 6, 2, 64, 16, torch.bfloat16)
+    torch.full_like(q, 7.0, memory_format=torch.contiguous_format)
+    out, _ = T.rope_append_paged(q, k, v, freq, kp, vp, table, torch.tensor(cu, device=DEV).to(torch.int32), kv_len, 4)
+    assert torch.isfinite(out).all() and (out != 7).all()
