@@ -3,6 +3,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -112,3 +115,33 @@ def test_options_that_are_not_known_are_refused():
         assert L.lib().tasft_rope_append_paged_opt(C.byref(a), options, None) == -1
         assert L.lib().tasft_bsa_chunk_paged_fwd_opt(C.byref(chunk_args()), options, None) == -1
     assert L.lib().tasft_rope_append_paged_opt(None, 0, None) == L.lib().tasft_bsa_chunk_paged_fwd_opt(None, 0, None) == -1
+
+
+@pytest.mark.parametrize("cname,pyname", [("tasft_rope_append_args", "RopeAppendArgs"), ("tasft_select_args", "SelectArgs"),
+                                          ("tasft_chunk_args", "ChunkArgs")])
+def test_argument_blocks_match_the_header(tmp_path, cname, pyname):
+    """Fields where the compiler lays them out, as ctypes and as packed bytes."""
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("gcc not available")
+    cls = getattr(L, pyname)
+    header = Path(L.__file__).resolve().parent.parent / "include" / "tasft_b200.h"
+    lines = ["#include <stddef.h>", "#include <stdio.h>", f'#include "{header}"', "int main(void) {",
+             f'  printf("%zu\\n", sizeof({cname}));']
+    lines += [f'  printf("%zu\\n", offsetof({cname}, {name}));' for name, _ in cls._fields_] + ["  return 0;", "}"]
+    (tmp_path / "layout.c").write_text("\n".join(lines))
+    exe = tmp_path / "layout"
+    subprocess.run([gcc, "-std=c11", "-o", str(exe), str(tmp_path / "layout.c")], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [C.sizeof(cls)] + [getattr(cls, name).offset for name, _ in cls._fields_]
+    values, block, n = [], cls(), 0
+    for name, kind in cls._fields_:
+        many = getattr(kind, "_length_", 0)
+        mine = [n + i + 1 for i in range(max(many, 1))]
+        n += len(mine)
+        values += mine
+        if many:
+            getattr(block, name)[:] = mine
+        else:
+            setattr(block, name, mine[0])
+    assert L.packed(cls)(*values) == bytes(block)
