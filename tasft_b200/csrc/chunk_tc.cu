@@ -36,10 +36,12 @@
 // holds keys that some row of the tile must not see, values that are not finite go to zero too,
 // and the rows that do see them take the infinity or NaN in the epilogue. Warp 3 does both while
 // the softmax of the block is under way.
-// Measured on a B200 (in a graph): 2048 tokens over 16384 cached ones, 32/8 heads, D 128, 493 us =
-// 1.18 PFLOP/s, held by the chain S -> softmax -> P.V of the two tiles an SM has in flight (tensor
-// pipe and MUFU half busy each) and by N64 tiles; 64 single tokens with 26 kept blocks in 16-token
-// pages 80 us = 5.4 TB/s, HBM; one token over 4000, 17 us, start (7 us) and merge launch (4 us).
+// Measured on B200s (in a graph): 2048 tokens over 16384 cached ones, 32/8 heads, D 128, 493 to 576
+// us = 1.18 to 1.02 PFLOP/s (the latter under the power cap), held by the chain S -> softmax -> P.V
+// of the two tiles an SM has in flight (tensor pipe and MUFU half busy each); 64 single tokens with
+// 26 kept blocks in 16-token pages 80 to 84 us = 5.1 to 5.4 TB/s, HBM; one token over 4000 17 us: 4
+// for a launch that finds no token, 6 for a first tile, 2 for the merge's launch, 5 for four blocks
+// a CTA and the merge.
 // Every mbarrier phase is indexed by a global counter and every wait is arranged so the waiter
 // is at most one phase behind; every wait is bounded (TASFT_DEVERR_TIMEOUT).
 #include "chunk.cuh"

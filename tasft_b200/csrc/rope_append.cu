@@ -16,9 +16,9 @@
 //
 // Bound by HBM: every row is read and written once. One CTA of 4 warps takes one 64-token block
 // of one sequence and as many of its heads; a warp takes a head, lanes over (16-byte column
-// pairs x rows), and holds the block sums in registers. Measured on a B200: 8192 tokens of 28/4
-// heads, D 128, 33 us = 4.4 TB/s (35 us without the trigonometry: the memory path); 64 tokens 9 us,
-// a chain of table, cos and sin and rows.
+// pairs x rows), and holds the block sums in registers. Measured on a B200: 7695 tokens of 28/4
+// heads, D 128, 32 us = 4.5 TB/s (no less without the trigonometry: loads and stores in flight); 64
+// tokens 9 us, a chain of table, cached rows, cos and sin, and new rows.
 #include "common.cuh"
 
 namespace tasft {

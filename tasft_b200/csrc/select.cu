@@ -12,7 +12,7 @@
 //
 // kT threads per row, kV values per thread (value v of thread t is block v * kT + t, so loads
 // are coalesced and a warp's ballot is one word of the bit rows). The scores are read once, 64 MB
-// for 2064 rows of up to 2048 blocks and 7 heads: 25 us on a B200 (9.8 at the copy rate), bound by
+// for 2064 rows of up to 1535 blocks and 7 heads: 24 us on a B200 (9.8 at the copy rate), bound by
 // issue (1,067 instructions a warp, slots 61% busy) and the chain of loads and barriers; 512 short rows 5 us.
 #include "common.cuh"
 
@@ -311,6 +311,9 @@ extern "C" int tasft_select_blocks(const tasft_select_args* ap, tasft_stream_t s
   const int64_t most = a.first + (int64_t)a.local > a.top_k ? a.first + (int64_t)a.local : a.top_k;
   if (a.width < (most < a.NBk ? most : a.NBk)) return TASFT_ERR_INVALID_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  // by the width of the scores (the rows' own lengths are on the device). At 1535 blocks 64 to 512
+  // threads a row took 27 to 39 us where 256 took 24 to 27; the widest spills 280 bytes (2064 rows of
+  // up to 4158 blocks: 315 us)
   if (a.NBk <= 128) return run<32, 4>(a, st);
   if (a.NBk <= 512) return run<128, 4>(a, st);
   if (a.NBk <= 2048) return run<256, 8>(a, st);
